@@ -17,8 +17,9 @@
 // dealt out in equal contiguous ranges, one per SM, worked out from the lengths on the device: every SM has the same
 // number of bytes to read, and a block goes from one sequence to the next without its ring running dry.
 #include <algorithm>
+#include <climits>
 
-#include "cwk_common.cuh"
+#include "gqa_steps.cuh"
 
 namespace {
 
@@ -29,82 +30,13 @@ constexpr float GQ_LAZY = 8.f;        // a score may outrun the reference expone
 struct GqaDecodeParams {
     const uint16_t *q, *k, *v;        // q bf16 [B][nh][hd]; caches: sequence b at + b * seq_stride, rows of ld
     int64_t seq_stride, ld;
-    const int32_t *kv_len, *sel;      // [B]; optional row lists [B][sel_ld]
+    const int32_t *sel;               // optional row lists [B][sel_ld]
     int64_t sel_ld;
-    int B, nh, nkv, group, hb;        // hb: KV heads a block works on at once (4, 2 or 1)
+    int nh, nkv, group, hb;           // hb: KV heads a block works on at once (4, 2 or 1)
     float scale_log2;
     float *rec;                       // [slot][warp][group][hd + 2]
-    int2 *meta;                       // [B][nkv / hb]: first slot, number of slots
+    GqaSteps steps;                   // groups: nkv / hb; keys: GK * (GW / hb)
 };
-
-// A block's place in the list of all steps: sequence, group of KV heads, step within it.
-struct GqaPlace {
-    int b, hg, step, steps, len;      // steps: of this sequence (and head group)
-};
-__device__ __forceinline__ int steps_of(const GqaDecodeParams &p, int b) { return b < p.B ? (max(p.kv_len[b], 0) + GK * (GW / p.hb) - 1) / (GK * (GW / p.hb)) : 0; }
-
-// This block's range [lo, hi) of all steps, and where it begins. Every warp works it out for itself; the first one notes, for
-// every (sequence, head group) whose first step is in the range, its first record slot (slots are numbered by head group
-// plus block: one of the two grows from record to record) and their number.
-__device__ __forceinline__ int gqa_range(const GqaDecodeParams &p, int lane, bool note, GqaPlace &at) {
-    const int nhg = p.nkv / p.hb;
-    int64_t total = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-        int v = steps_of(p, b0 + lane);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        total += v;
-    }
-    total *= nhg;
-    const int64_t G = max((int64_t)1, min((int64_t)gridDim.x, total)), g = blockIdx.x;      // no block between two others is left without a step
-    const int64_t lo = g < G ? total * g / G : total, hi = g < G ? total * (g + 1) / G : total;
-    int64_t before = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-        const int mine = steps_of(p, b0 + lane);
-        int v = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += u;
-        }
-        const int64_t s0 = (before + v - mine) * nhg, s1 = s0 + (int64_t)mine * nhg;       // this lane's sequence: steps [s0, s1)
-        const bool here = mine > 0 && s0 <= lo && lo < s1 && lo < hi;
-        const uint32_t who = __ballot_sync(0xffffffffu, here);
-        if (who) {
-            const int src = __ffs(who) - 1;
-            at.b = b0 + src;
-            at.steps = __shfl_sync(0xffffffffu, mine, src);
-            const int off = (int)__shfl_sync(0xffffffffu, (int)(lo - s0), src);
-            at.hg = off / at.steps;
-            at.step = off % at.steps;
-        }
-        if (note && b0 + lane < p.B) {
-            if (mine == 0) {
-                if (s0 > 0 ? (lo < s0 && s0 <= hi) : g == 0)
-                    for (int h = 0; h < nhg; h++) p.meta[(b0 + lane) * nhg + h] = make_int2(0, 0);
-            } else if (s0 < hi && s1 > lo) {
-                const int64_t h0 = lo > s0 ? (lo - s0 + mine - 1) / mine : 0;              // first head group that begins here
-                for (int64_t h = h0; h < nhg && s0 + h * mine < hi; h++) {
-                    const int64_t g1 = ((s0 + (h + 1) * mine) * G - 1) / total;              // the block with its last step
-                    p.meta[(b0 + lane) * nhg + h] = make_int2((int)((b0 + lane) * nhg + h + g), (int)(g1 - g + 1));
-                }
-            }
-        }
-        before += __shfl_sync(0xffffffffu, v, 31);
-    }
-    return (int)(hi - lo);
-}
-__device__ __forceinline__ void gqa_advance(const GqaDecodeParams &p, GqaPlace &at) {      // to the next step; there is one
-    if (++at.step < at.steps) return;
-    at.step = 0;
-    if (++at.hg < p.nkv / p.hb) return;
-    at.hg = 0;
-    do {
-        at.b++;
-        at.len = p.kv_len[at.b];
-    } while (at.len <= 0);
-    at.steps = steps_of(p, at.b);
-}
 
 template <int HD>
 __global__ void __launch_bounds__(32 * GW) gqa_decode_kernel(const GqaDecodeParams p) {
@@ -115,13 +47,13 @@ __global__ void __launch_bounds__(32 * GW) gqa_decode_kernel(const GqaDecodePara
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
     const uint32_t ring = smem_u32(smem) + warp * STAGES * 2 * KB;
     const int sub = warp / p.hb, wh = warp % p.hb;        // which sixteen keys of a step, which KV head of the group
-    const int keys = GK * (GW / p.hb);
+    const int keys = p.steps.keys;
     GqaPlace at{0, 0, 0, 0, 0};
     cwk_pdl_launch();
     cwk_pdl_wait();
-    const int n = gqa_range(p, lane, warp == 0, at);
+    const int n = gqa_range(p.steps, lane, warp == 0, at);
     if (n <= 0) return;
-    at.len = p.kv_len[at.b];
+    at.len = length_of(p.steps, at.b);
     GqaPlace ld = at;                                     // the step being loaded
     auto load = [&](int slot) {
         const int j0 = ld.step * keys + sub * GK, kvh = ld.hg * p.hb + wh;
@@ -144,7 +76,7 @@ __global__ void __launch_bounds__(32 * GW) gqa_decode_kernel(const GqaDecodePara
     for (int s = 0; s < STAGES - 1; s++) {
         if (s < n) {
             load(s);
-            if (s + 1 < n) gqa_advance(p, ld);
+            if (s + 1 < n) gqa_advance(p.steps, ld);
         }
         cp_async_commit();
     }
@@ -167,7 +99,7 @@ __global__ void __launch_bounds__(32 * GW) gqa_decode_kernel(const GqaDecodePara
         __syncwarp();                                     // every lane's copies of this step have landed; the last step's slot has been read
         if (s + STAGES - 1 < n) {
             load((s + STAGES - 1) % STAGES);
-            if (s + STAGES < n) gqa_advance(p, ld);
+            if (s + STAGES < n) gqa_advance(p.steps, ld);
         }
         cp_async_commit();
         const uint32_t tK = ring + (s % STAGES) * 2 * KB, tV = tK + KB;
@@ -240,74 +172,32 @@ __global__ void __launch_bounds__(32 * GW) gqa_decode_kernel(const GqaDecodePara
                 if (h0 + 1 < p.group) { o[(h0 + 1) * (HD + 2)] = acc[i][1]; o[(h0 + 1) * (HD + 2) + 8] = acc[i][3]; }
             }
         }
-        if (s + 1 < n) gqa_advance(p, at);
+        if (s + 1 < n) gqa_advance(p.steps, at);
     }
     cp_async_wait<0>();
 }
 
-// grid (query head, sequence), (HD / 2) x GROUPS threads: two columns each, the records of the head's blocks and warps dealt
-// out to the groups (one sequence has a record from every block: 148 in a row are 20 us of loads for one group of threads).
+// grid (query head, sequence), (HD / 2) x GROUPS threads (gqa_merge_records)
 template <int HD, int GROUPS>
 __global__ void __launch_bounds__(HD / 2 * GROUPS) gqa_merge_kernel(const GqaDecodeParams p, uint16_t *out) {
-    constexpr int NT = HD / 2;
-    __shared__ float s_m[GROUPS], s_l[GROUPS];
-    __shared__ float2 s_o[GROUPS][NT];
     const int h = blockIdx.x, b = blockIdx.y, kvh = h / p.group, nhg = p.nkv / p.hb, ks = GW / p.hb;
-    const int g = threadIdx.x / NT, tid = threadIdx.x % NT;
+    const int tid = threadIdx.x % (HD / 2);
     cwk_pdl_launch();
     cwk_pdl_wait();
-    const int2 meta = p.meta[b * nhg + kvh / p.hb];
+    const int2 meta = p.steps.meta[b * nhg + kvh / p.hb];
     const int64_t rsz = (int64_t)p.group * (HD + 2);
     // record i: slot first + i / ks, warp (i % ks) * hb + kvh % hb
     const float *base = p.rec + ((int64_t)meta.x * GW + kvh % p.hb) * rsz + (int64_t)(h % p.group) * (HD + 2);
-    const int cnt = meta.y * ks;
     auto at = [&](int i) { return base + (ks == 1 ? (int64_t)i * GW : (int64_t)(i / ks) * GW + (i % ks) * p.hb) * rsz; };
-    float M = -INFINITY, den = 0.f, x = 0.f, y = 0.f;
-    for (int i0 = g; i0 < cnt; i0 += 8 * GROUPS) {         // eight records' loads at once; the running maximum as the scores'
-        float m[8], l[8];
-        float2 o[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int i = i0 + j * GROUPS;
-            const float *r = at(min(i, cnt - 1));
-            m[j] = i < cnt ? r[0] : -INFINITY;
-            l[j] = r[1];
-            o[j] = *reinterpret_cast<const float2 *>(r + 2 + 2 * tid);
-        }
-        float mx = M;
-#pragma unroll
-        for (int j = 0; j < 8; j++) mx = fmaxf(mx, m[j]);
-        if (mx == -INFINITY) continue;
-        const float a = exp2f(M - mx);
-        den *= a; x *= a; y *= a;
-        M = mx;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float w = exp2f(m[j] - M);
-            den += w * l[j]; x += w * o[j].x; y += w * o[j].y;
-        }
-    }
-    if (GROUPS > 1) {
-        if (tid == 0) { s_m[g] = M; s_l[g] = den; }
-        s_o[g][tid] = make_float2(x, y);
-        __syncthreads();
-        if (g > 0) return;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < GROUPS; j++) mx = fmaxf(mx, s_m[j]);
-        den = x = y = 0.f;
-#pragma unroll
-        for (int j = 0; j < GROUPS; j++) {
-            const float w = s_m[j] == -INFINITY ? 0.f : exp2f(s_m[j] - mx);
-            den += w * s_l[j]; x += w * s_o[j][tid].x; y += w * s_o[j][tid].y;
-        }
-    }
+    float den, x, y;
+    if (!gqa_merge_records<HD, GROUPS>(meta.y * ks, at, den, x, y)) return;
     const float inv = den > 0.f ? 1.f / den : 0.f;
     *reinterpret_cast<uint32_t *>(out + ((int64_t)b * p.nh + h) * HD + 2 * tid) = pack_bf16x2(x * inv, y * inv);
 }
 
 template <int HD>
 int launch(cwk_ctx *ctx, const GqaDecodeParams &p, int blocks, void *out) {
+    const int B = p.steps.B;
     constexpr int SMEM = GW * (HD == 256 ? 3 : 6) * 2 * GK * HD * 2;      // 192 KB
     static bool attr_set[16] = {false};
     if (!attr_set[ctx->device & 15]) {
@@ -319,8 +209,8 @@ int launch(cwk_ctx *ctx, const GqaDecodeParams &p, int blocks, void *out) {
         CWK_CUDA(ctx, cwk_launch_early(gqa_decode_kernel<HD>, dim3(blocks), dim3(32 * GW), SMEM, ctx->stream, p));
         ctx->launches++;
     }
-    const bool many = (int64_t)blocks * (GW / p.hb) * (p.nkv / p.hb) > 8 * (int64_t)p.B * (p.nkv / p.hb);      // records per head and sequence
-    CWK_CUDA(ctx, cwk_launch_early(many ? gqa_merge_kernel<HD, 8> : gqa_merge_kernel<HD, 1>, dim3(p.nh, p.B), dim3(HD / 2 * (many ? 8 : 1)), 0, ctx->stream, p, (uint16_t *)out));
+    const bool many = (int64_t)blocks * (GW / p.hb) * (p.nkv / p.hb) > 8 * (int64_t)B * (p.nkv / p.hb);      // records per head and sequence
+    CWK_CUDA(ctx, cwk_launch_early(many ? gqa_merge_kernel<HD, 8> : gqa_merge_kernel<HD, 1>, dim3(p.nh, B), dim3(HD / 2 * (many ? 8 : 1)), 0, ctx->stream, p, (uint16_t *)out));
     ctx->launches++;
     return CWK_OK;
 }
@@ -332,7 +222,7 @@ int cwk_gqa_decode_streams(cwk_ctx *ctx, const void *q, const void *K, const voi
                            const int32_t *sel, int64_t sel_ld, int B, int nh, int nkv, int hd, float scale, void *out, int max_blocks) {
     GqaDecodeParams p;
     p.q = (const uint16_t *)q; p.k = (const uint16_t *)K; p.v = (const uint16_t *)V; p.seq_stride = seq_stride; p.ld = (int64_t)nkv * hd;
-    p.kv_len = kv_len; p.sel = sel; p.sel_ld = sel_ld; p.B = B; p.nh = nh; p.nkv = nkv; p.group = nh / nkv;
+    p.sel = sel; p.sel_ld = sel_ld; p.nh = nh; p.nkv = nkv; p.group = nh / nkv;
     p.hb = nkv % 4 == 0 ? 4 : nkv % 2 == 0 ? 2 : 1;
     p.scale_log2 = scale * 1.4426950408889634f;
     // as many blocks as there can be steps, at most one per SM
@@ -344,6 +234,6 @@ int cwk_gqa_decode_streams(cwk_ctx *ctx, const void *q, const void *K, const voi
     int s = cwk_reserve_scratch(ctx, rec_bytes + (size_t)B * (nkv / p.hb) * sizeof(int2));
     if (s != CWK_OK) return s;
     p.rec = ctx->scratch;
-    p.meta = (int2 *)((uint8_t *)ctx->scratch + rec_bytes);
+    p.steps = GqaSteps{kv_len, B, nkv / p.hb, keys, INT_MAX - 256, (int2 *)((uint8_t *)ctx->scratch + rec_bytes)};
     return hd == 256 ? launch<256>(ctx, p, blocks, out) : launch<128>(ctx, p, blocks, out);
 }
