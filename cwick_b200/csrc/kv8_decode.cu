@@ -1,0 +1,373 @@
+// kv8_decode.cu -- GQA decode over a cache held in 8 bits (kv8.cuh), for a batch of sequences with lengths of their own and one or a few
+// query tokens each, and the entry of the prompt chunk over such a cache.
+//
+// The streams of gqa_decode.cu over half the bytes: no warp waits for another one, every warp has a ring of its own (32 keys a stage, K and V
+// codes, filled by asynchronous copies), its own running maximum, sum and output, and the steps of all sequences are dealt out in equal
+// contiguous ranges (gqa_steps.cuh). Codes become f16 in registers, exactly, on the way into mma.m16n8k16 (f16 operands, f32 sums), keys or
+// value columns as its sixteen rows, query rows as its eight columns:
+//   scores   a lane's 4 neighbouring bytes of a key are the MMA's k positions 2t, 2t+1, 2t+8, 2t+9: the dims are only renumbered, for
+//            the queries alike, and no byte moves.
+//   values   ldmatrix.trans on pairs of bytes gives a lane two keys of two neighbouring columns; one byte permutation pairs the keys, and
+//            the even column goes to row g of the MMA, the odd one to row g + 8.
+// The queries go to f16 too: each row divided by a power of two that brings its largest value into [1, 2), so what is lost is below
+// 2^-25 of that value, 2^-16 of a bf16 step. Probabilities are f16 in [0, 2^8], three bits finer than bf16's; their sums are f32. The
+// scales are powers of two: a step's 32 keys are in one block, the key scale multiplies its scores and the value scale its product
+// on the way into the f32 accumulators, so no code's value is ever rounded or out of f16's range.
+#include <algorithm>
+
+#include "gqa_steps.cuh"
+#include "kv8.cuh"
+
+namespace {
+
+constexpr int GW = 4;                 // warps per block
+constexpr int GK = 32;                // keys per warp and step; every block of the cache is a multiple of it
+constexpr float GQ_LAZY = 8.f;        // a score may outrun the reference exponent by 2^8 before a rescale
+
+struct Kv8DecodeParams {
+    const uint16_t *q;                // bf16 [B][n][nh][hd]
+    const uint8_t *k, *v, *ks, *vs;
+    int64_t rows;                     // per slot
+    int n, nh, nkv, group, hb, lb;    // hb: KV heads a block works on at once (4, 2 or 1); block = 1 << lb
+    int per, parts;                   // query tokens whose heads share the MMA columns; parts = ceil(n / per)
+    float scale_log2;
+    float *rec;                       // [slot][warp][per * group][hd + 2]
+    GqaSteps steps;                   // groups: (nkv / hb) * parts, the parts of the same keys next to each other; keys: GK * (GW / hb)
+};
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+template <int HD> constexpr int KV8_STAGES = HD == 256 ? 3 : 6;
+
+// NB: groups of eight MMA columns (query rows)
+template <int HD, int NB, bool I8>
+__global__ void __launch_bounds__(32 * GW) kv8_decode_kernel(const Kv8DecodeParams p) {
+    constexpr int CH = HD / 16;                           // 16-byte pieces per row
+    constexpr int STAGES = KV8_STAGES<HD>;
+    constexpr int KB = GK * HD;                           // bytes of a stage's K (and of its V)
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
+    const uint32_t ring = smem_u32(smem) + warp * STAGES * 2 * KB;
+    const int sub = warp / p.hb, wh = warp % p.hb;        // which 32 keys of a step, which KV head of the group
+    const int keys = p.steps.keys, cols = p.per * p.group;
+    GqaPlace at{0, 0, 0, 0, 0};
+    cwk_pdl_launch();
+    cwk_pdl_wait();
+    const int n = gqa_range(p.steps, lane, warp == 0, at);
+    if (n <= 0) return;
+    at.len = length_of(p.steps, at.b);
+    GqaPlace ld = at;                                     // the step being loaded
+    auto head_of = [&](const GqaPlace &x) { return (x.hg / p.parts) * p.hb + wh; };
+    auto load = [&](int slot) {
+        const int j0 = ld.step * keys + sub * GK;
+        const int64_t row = (int64_t)p.nkv * HD, base = (int64_t)ld.b * p.rows * row + head_of(ld) * HD;
+        const uint32_t dst = ring + slot * 2 * KB;
+        constexpr int RPI = 32 / CH;                      // rows per instruction: 2 or 4
+        const int c = lane % CH, rr = lane / CH;
+#pragma unroll
+        for (int i = 0; i < GK / RPI; i++) {
+            const int r = i * RPI + rr;
+            const bool ok = j0 + r < ld.len;              // (rows behind the last are not read: zeros in their place)
+            const int64_t off = base + (ok ? (int64_t)(j0 + r) * row : 0) + c * 16;
+            const uint32_t d = dst + r * HD + ((c ^ (r & 7)) << 4);
+            cp_async16(d, p.k + off, ok);
+            cp_async16(d + KB, p.v + off, ok);
+        }
+    };
+    // the two scales of this warp's keys at a place (any value where it has no key there)
+    auto scales = [&](const GqaPlace &x) -> uint32_t {
+        const int j0 = x.step * keys + sub * GK;
+        if (j0 >= x.len) return 127u | 127u << 8;
+        const int64_t i = ((int64_t)x.b * (p.rows >> p.lb) + (j0 >> p.lb)) * p.nkv + head_of(x);
+        return (uint32_t)p.ks[i] | (uint32_t)p.vs[i] << 8;
+    };
+    for (int s = 0; s < STAGES - 1; s++) {
+        if (s < n) {
+            load(s);
+            if (s + 1 < n) gqa_advance(p.steps, ld);
+        }
+        cp_async_commit();
+    }
+    uint32_t bq[HD / 16][NB][2];                          // the query rows, as the score MMAs' second operand
+    float acc[HD / 16][NB][4];                            // value columns 16 i + 2 lg (+ 1) of query rows 8 nb + 2 lt, + 1
+    float m[NB][2], l[NB][2], unit[NB][2];                // unit: what a score MMA's result is multiplied by, besides the key scale
+    int limit[NB][2];                                     // rows that the query row sees
+    uint32_t sc = scales(at);
+    bool fresh = true;
+    for (int s = 0; s < n; s++) {
+        if (fresh) {
+            const int part = at.hg % p.parts;
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                // this lane's dims of query row 8 nb + lg: 16 i + 4 lt .. + 3
+                const int col = nb * 8 + lg, tok = part * p.per + col / p.group;
+                const bool on = col < cols && tok < p.n;
+                const uint16_t *qr = p.q + (((int64_t)at.b * p.n + tok) * p.nh + head_of(at) * p.group + col % p.group) * HD + 4 * lt;
+                uint2 u[HD / 16];
+                float big = 0.f;
+#pragma unroll
+                for (int i = 0; i < HD / 16; i++) {
+                    u[i] = on ? *reinterpret_cast<const uint2 *>(qr + i * 16) : make_uint2(0u, 0u);
+                    big = fmaxf(fmaxf(big, fmaxf(fabsf(__uint_as_float(u[i].x << 16)), fabsf(__uint_as_float(u[i].x & 0xFFFF0000u)))),
+                                fmaxf(fabsf(__uint_as_float(u[i].y << 16)), fabsf(__uint_as_float(u[i].y & 0xFFFF0000u))));
+                }
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                const int e = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 120);
+                const float down = kv8_two(-e);
+#pragma unroll
+                for (int i = 0; i < HD / 16; i++) {
+                    bq[i][nb][0] = pack_f16x2(__uint_as_float(u[i].x << 16) * down, __uint_as_float(u[i].x & 0xFFFF0000u) * down);
+                    bq[i][nb][1] = pack_f16x2(__uint_as_float(u[i].y << 16) * down, __uint_as_float(u[i].y & 0xFFFF0000u) * down);
+                    acc[i][nb][0] = acc[i][nb][1] = acc[i][nb][2] = acc[i][nb][3] = 0.f;
+                }
+                // the two rows whose scores this lane gets are those of lanes with lg = 2 lt, 2 lt + 1
+                const float up = kv8_two(e) * p.scale_log2;
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    unit[nb][x] = __shfl_sync(0xffffffffu, up, (2 * lt + x) * 4);
+                    limit[nb][x] = at.len - (p.n - 1 - (part * p.per + (nb * 8 + 2 * lt + x) / p.group));
+                    l[nb][x] = 0.f;
+                }
+            }
+        }
+        cp_async_wait<STAGES - 2>();
+        __syncwarp();                                     // every lane's copies of this step have landed; the last step's slot has been read
+        if (s + STAGES - 1 < n) {
+            load((s + STAGES - 1) % STAGES);
+            if (s + STAGES < n) gqa_advance(p.steps, ld);
+        }
+        cp_async_commit();
+        GqaPlace next = at;                               // its scales are asked for a step ahead
+        uint32_t sc_next = 0;
+        if (s + 1 < n) {
+            gqa_advance(p.steps, next);
+            sc_next = scales(next);
+        }
+        const uint32_t tK = ring + (s % STAGES) * 2 * KB, tV = tK + KB;
+        const uint32_t row = lane * HD, x7 = lane & 7;    // ldmatrix: a lane's address is key `lane`'s
+        const float kscale = kv8_scale(sc & 255u), vscale = kv8_scale(sc >> 8);
+        float c[2][NB][4];                                // scores of keys 16 h + lg, + 8
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) c[h][nb][0] = c[h][nb][1] = c[h][nb][2] = c[h][nb][3] = 0.f;
+#pragma unroll
+        for (int i = 0; i < HD / 16; i++) {
+            uint32_t r[4], a[2][4];
+            ldmatrix_x4(r[0], r[1], r[2], r[3], tK + row + ((i ^ x7) << 4));
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                kv8_decode4<I8>(r[2 * h], a[h][0], a[h][2]);
+                kv8_decode4<I8>(r[2 * h + 1], a[h][1], a[h][3]);
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) mma_f16_16816(c[h][nb], a[h], bq[i][nb][0], bq[i][nb][1]);
+            }
+        }
+        const int j0 = at.step * keys + sub * GK + lg;    // this lane's keys: j0, + 8, + 16, + 24
+        uint32_t b[2][NB][2];                             // the probabilities, as the value MMAs' second operand
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            float t[4][2];
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)               // (one factor after the other: their product alone may be out of range)
+                    t[k][x] = j0 + 8 * k < limit[nb][x] ? c[k >> 1][nb][(k & 1) * 2 + x] * unit[nb][x] * kscale : -INFINITY;
+            float big[2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) big[x] = fmaxf(fmaxf(t[0][x], t[1][x]), fmaxf(t[2][x], t[3][x]));
+            if (fresh || __any_sync(0xffffffffu, big[0] > m[nb][0] + GQ_LAZY || big[1] > m[nb][1] + GQ_LAZY)) {
+#pragma unroll
+                for (int x = 0; x < 2; x++)
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) big[x] = fmaxf(big[x], __shfl_xor_sync(0xffffffffu, big[x], o));
+                if (fresh) {                              // (a row that sees none of these keys sees none behind them: any exponent will do)
+                    m[nb][0] = big[0] == -INFINITY ? 0.f : big[0];
+                    m[nb][1] = big[1] == -INFINITY ? 0.f : big[1];
+                } else {
+                    float f[2];
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const float to = fmaxf(m[nb][x], big[x]);
+                        f[x] = exp2f(m[nb][x] - to);
+                        m[nb][x] = to;
+                        l[nb][x] *= f[x];
+                    }
+#pragma unroll
+                    for (int i = 0; i < HD / 16; i++) { acc[i][nb][0] *= f[0]; acc[i][nb][1] *= f[1]; acc[i][nb][2] *= f[0]; acc[i][nb][3] *= f[1]; }
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) t[k][x] = exp2f(t[k][x] - m[nb][x]);
+                l[nb][x] += (t[0][x] + t[1][x]) + (t[2][x] + t[3][x]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {                 // [8 keys][8 rows] each -> [8 rows][8 keys]
+                uint32_t &w = b[k >> 1][nb][k & 1];
+                w = pack_f16x2(t[k][0], t[k][1]);
+                asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(w));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < HD / 16; i++) {
+            uint32_t r[4], a[2][4];
+            ldmatrix_x4_trans(r[0], r[1], r[2], r[3], tV + row + ((i ^ x7) << 4));
+            float d[NB][4];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) d[nb][0] = d[nb][1] = d[nb][2] = d[nb][3] = 0.f;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                kv8_decode4_even_odd<I8>(r[2 * h], a[h][0], a[h][1]);
+                kv8_decode4_even_odd<I8>(r[2 * h + 1], a[h][2], a[h][3]);
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) mma_f16_16816(d[nb], a[h], b[h][nb][0], b[h][nb][1]);
+            }
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int x = 0; x < 4; x++) acc[i][nb][x] = fmaf(d[nb][x], vscale, acc[i][nb][x]);
+        }
+        fresh = at.step + 1 == at.steps;
+        if (fresh || s + 1 == n) {                        // the end of what this block has of the sequence's head group: its record
+            const int64_t slot = (int64_t)at.b * p.steps.groups + at.hg + blockIdx.x;
+            float *rec = p.rec + (slot * GW + warp) * cols * (HD + 2);
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    float sum = l[nb][x];
+#pragma unroll
+                    for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    const int col = nb * 8 + 2 * lt + x;
+                    if (col >= cols) continue;
+                    float *o = rec + col * (HD + 2);
+                    if (lg == 0) *reinterpret_cast<float2 *>(o) = make_float2(sum != 0.f ? m[nb][x] : -INFINITY, sum);
+#pragma unroll
+                    for (int i = 0; i < HD / 16; i++)
+                        *reinterpret_cast<float2 *>(o + 2 + i * 16 + 2 * lg) = make_float2(acc[i][nb][x], acc[i][nb][2 + x]);
+                }
+        }
+        at = next;
+        sc = sc_next;
+    }
+    cp_async_wait<0>();
+}
+
+// grid (query row = token x head, sequence), (HD / 2) x GROUPS threads (gqa_merge_records)
+template <int HD, int GROUPS>
+__global__ void __launch_bounds__(HD / 2 * GROUPS) kv8_merge_kernel(const Kv8DecodeParams p, uint16_t *out) {
+    const int tok = blockIdx.x / p.nh, h = blockIdx.x % p.nh, b = blockIdx.y, kvh = h / p.group, ks = GW / p.hb, cols = p.per * p.group;
+    const int tid = threadIdx.x % (HD / 2);
+    cwk_pdl_launch();
+    cwk_pdl_wait();
+    const int2 meta = p.steps.meta[b * p.steps.groups + (kvh / p.hb) * p.parts + tok / p.per];
+    const int64_t rsz = (int64_t)cols * (HD + 2);
+    // record i: slot first + i / ks, warp (i % ks) * hb + kvh % hb
+    const float *base = p.rec + ((int64_t)meta.x * GW + kvh % p.hb) * rsz + (int64_t)((tok % p.per) * p.group + h % p.group) * (HD + 2);
+    auto at = [&](int i) { return base + (ks == 1 ? (int64_t)i * GW : (int64_t)(i / ks) * GW + (i % ks) * p.hb) * rsz; };
+    float den, x, y;
+    if (!gqa_merge_records<HD, GROUPS>(meta.y * ks, at, den, x, y)) return;
+    const float inv = den != 0.f ? 1.f / den : 0.f;
+    *reinterpret_cast<uint32_t *>(out + (((int64_t)b * p.n + tok) * p.nh + h) * HD + 2 * tid) = pack_bf16x2(x * inv, y * inv);
+}
+
+template <int HD, int NB>
+int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *out) {
+    constexpr int SMEM = GW * KV8_STAGES<HD> * 2 * GK * HD;      // 192 KB
+    const bool i8 = type == CWK_KV8_INT8;
+    auto kern = i8 ? kv8_decode_kernel<HD, NB, true> : kv8_decode_kernel<HD, NB, false>;
+    static bool attr_set[2][16] = {};
+    if (!attr_set[i8][ctx->device & 15]) {
+        CWK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        attr_set[i8][ctx->device & 15] = true;
+    }
+    {
+        CwkKernelTimer timer(ctx);
+        CWK_CUDA(ctx, cwk_launch_early(kern, dim3(blocks), dim3(32 * GW), SMEM, ctx->stream, p));
+        ctx->launches++;
+    }
+    const bool many = (int64_t)blocks * (GW / p.hb) > 8 * (int64_t)p.steps.B * p.parts;      // records per query row
+    CWK_CUDA(ctx, cwk_launch_early(many ? kv8_merge_kernel<HD, 8> : kv8_merge_kernel<HD, 1>, dim3(p.n * p.nh, p.steps.B), dim3(HD / 2 * (many ? 8 : 1)), 0,
+                                   ctx->stream, p, (uint16_t *)out));
+    ctx->launches++;
+    return CWK_OK;
+}
+
+}  // namespace
+
+int cwk_kv8_streams(cwk_ctx *ctx, const void *q, const cwk_kv8 &c, const int32_t *kv_len, int max_kv_len, int B, int n, int nh, float scale,
+                    void *out, int max_blocks) {
+    Kv8DecodeParams p{};
+    p.q = (const uint16_t *)q; p.k = (const uint8_t *)c.k; p.v = (const uint8_t *)c.v; p.ks = c.k_scale; p.vs = c.v_scale; p.rows = c.rows;
+    p.n = n; p.nh = nh; p.nkv = c.nkv; p.group = nh / c.nkv; p.hb = c.nkv % 4 == 0 ? 4 : c.nkv % 2 == 0 ? 2 : 1;
+    p.lb = c.block == 32 ? 5 : c.block == 64 ? 6 : 7;
+    p.per = std::min(n, std::max(1, 16 / p.group));
+    p.parts = (n + p.per - 1) / p.per;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    // as many blocks as there can be steps, at most one per SM
+    const int keys = GK * (GW / p.hb);
+    const int64_t groups = (int64_t)(c.nkv / p.hb) * p.parts;
+    const int64_t most = std::max<int64_t>(1, B * groups * ((max_kv_len + keys - 1) / keys));
+    const int blocks = (int)std::min<int64_t>(most, max_blocks > 0 ? std::min(max_blocks, ctx->sm_count) : ctx->sm_count);
+    const size_t rec_bytes = (size_t)(B * groups + blocks) * GW * p.per * p.group * (c.hd + 2) * sizeof(float);
+    const int s = cwk_reserve_scratch(ctx, rec_bytes + (size_t)B * groups * sizeof(int2));
+    if (s != CWK_OK) return s;
+    p.rec = ctx->scratch;
+    p.steps = GqaSteps{kv_len, B, (int)groups, keys, kv_len ? (int)c.rows : max_kv_len, (int2 *)((uint8_t *)ctx->scratch + rec_bytes)};
+    if (p.per * p.group > 8) return c.hd == 256 ? launch<256, 2>(ctx, p, c.type, blocks, out) : launch<128, 2>(ctx, p, c.type, blocks, out);
+    return c.hd == 256 ? launch<256, 1>(ctx, p, c.type, blocks, out) : launch<128, 1>(ctx, p, c.type, blocks, out);
+}
+
+extern "C" {
+
+int cwk_gqa_decode_kv8(cwk_ctx *ctx, const void *q, const cwk_kv8 *c, const int32_t *kv_len, int max_kv_len, int B, int n, int nh, float scale,
+                       void *out, int n_splits) {
+    int s = cwk_kv8_check(ctx, c, "gqa_decode_kv8");
+    if (s != CWK_OK) return s;
+    if (!ctx || !q || !kv_len || !out) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_decode_kv8: null argument");
+    if (B <= 0 || B > 65535 || B > c->slots || n <= 0 || nh <= 0 || nh % c->nkv != 0 || max_kv_len < 0 || max_kv_len > c->rows)
+        return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_decode_kv8: bad dimensions");
+    if (nh / c->nkv > 16) return cwk_fail(ctx, CWK_ERR_UNSUPPORTED, "gqa_decode_kv8: group %d not built (up to 16)", nh / c->nkv);
+    if ((((uintptr_t)q | (uintptr_t)out) & 15) != 0) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_decode_kv8: pointers must be 16-byte aligned");
+    CWK_CUDA(ctx, cudaSetDevice(ctx->device));
+    return cwk_kv8_streams(ctx, q, *c, kv_len, max_kv_len, B, n, nh, scale, out,
+                           n_splits > 0 ? (int)std::min<int64_t>((int64_t)n_splits * B * c->nkv, 1 << 20) : 0);
+}
+
+int cwk_gqa_prefill_kv8(cwk_ctx *ctx, const void *Q, const cwk_kv8 *c, int slot, int64_t pos, int n, int nh, float scale, void *out) {
+    int s = cwk_kv8_check(ctx, c, "gqa_prefill_kv8");
+    if (s != CWK_OK) return s;
+    if (!ctx || !Q || !out) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_prefill_kv8: null argument");
+    if (slot < 0 || slot >= c->slots || n <= 0 || pos < 0 || pos > c->rows - n || nh <= 0 || nh % c->nkv != 0)
+        return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_prefill_kv8: bad dimensions");
+    const int group = nh / c->nkv;
+    if (group > 16 || 64 % group != 0) return cwk_fail(ctx, CWK_ERR_UNSUPPORTED, "gqa_prefill_kv8: group %d not built (1, 2, 4, 8, 16)", group);
+    if ((((uintptr_t)Q | (uintptr_t)out) & 15) != 0) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_prefill_kv8: pointers must be 16-byte aligned");
+    CWK_CUDA(ctx, cudaSetDevice(ctx->device));
+    // the slot's rows widened, exactly, behind the flags that the bf16 kernel keeps at the start of the workspace
+    cwk_kv8 at = *c;
+    const int64_t T = pos + n, row = (int64_t)c->nkv * c->hd;
+    at.k = (uint8_t *)c->k + slot * c->rows * row; at.v = (uint8_t *)c->v + slot * c->rows * row;
+    at.k_scale = c->k_scale + slot * (c->rows / c->block) * c->nkv; at.v_scale = c->v_scale + slot * (c->rows / c->block) * c->nkv;
+    const size_t flags = ((((size_t)((n + 127) / 128) * nh + ctx->sm_count + 3) * sizeof(int)) + 255) & ~(size_t)255, half = (size_t)T * row * 2;
+    s = cwk_reserve_work(ctx, flags + 2 * half);
+    if (s != CWK_OK) return s;
+    uint8_t *wk = (uint8_t *)ctx->work + flags;
+    s = cwk_kv8_widen(ctx, at, 0, T, wk, wk + half);
+    if (s != CWK_OK) return s;
+    return cwk_gqa_prefill(ctx, Q, wk, wk + half, pos, n, nh, c->nkv, c->hd, scale, out);
+}
+
+}  // extern "C"

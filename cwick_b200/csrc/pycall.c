@@ -57,8 +57,31 @@ WRAP(cwk_gdn_scan, 17, {
     RUN(cwk_gdn_scan(c, B, n_, nh, hk, hv, grp, up, gd, be, ga, al, dt, no, eps, S, out));
 })
 
+WRAP(cwk_kv8_store, 9, {
+    cwk_ctx *c = ptr(a[0]); void *cache = ptr(a[1]), *k = ptr(a[2]), *v = ptr(a[3]); const int f32_ = i32(a[4]);
+    void *pos = ptr(a[5]), *count = ptr(a[6]); const int B = i32(a[7]), n_ = i32(a[8]);
+    RUN(cwk_kv8_store(c, cache, k, v, f32_, pos, count, B, n_));
+})
+WRAP(cwk_kv8_load, 9, {
+    cwk_ctx *c = ptr(a[0]); void *cache = ptr(a[1]), *pos = ptr(a[2]), *count = ptr(a[3]); const int B = i32(a[4]), n_ = i32(a[5]);
+    void *k = ptr(a[6]), *v = ptr(a[7]); const int f32_ = i32(a[8]);
+    RUN(cwk_kv8_load(c, cache, pos, count, B, n_, k, v, f32_));
+})
+WRAP(cwk_gqa_qk_prep_kv8, 16, {
+    cwk_ctx *c = ptr(a[0]); void *qg = ptr(a[1]), *k = ptr(a[2]), *v = ptr(a[3]), *qn = ptr(a[4]), *kn = ptr(a[5]); const float eps = f32(a[6]);
+    const int rot = i32(a[7]); const double theta = PyFloat_AsDouble(a[8]); void *pos = ptr(a[9]), *count = ptr(a[10]);
+    const int B = i32(a[11]), n_ = i32(a[12]), nh = i32(a[13]); void *q_out = ptr(a[14]), *cache = ptr(a[15]);
+    RUN(cwk_gqa_qk_prep_kv8(c, qg, k, v, qn, kn, eps, rot, theta, pos, count, B, n_, nh, q_out, cache));
+})
+WRAP(cwk_gqa_decode_kv8, 11, {
+    cwk_ctx *c = ptr(a[0]); void *q = ptr(a[1]), *cache = ptr(a[2]), *len = ptr(a[3]); const int max_len = i32(a[4]), B = i32(a[5]), n_ = i32(a[6]);
+    const int nh = i32(a[7]); const float scale = f32(a[8]); void *out = ptr(a[9]); const int splits = i32(a[10]);
+    RUN(cwk_gqa_decode_kv8(c, q, cache, len, max_len, B, n_, nh, scale, out, splits));
+})
+
 static PyMethodDef methods[] = {
 #define M(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, NULL}
-    M(cwk_mla_decode), M(cwk_gqa_decode), M(cwk_dsa_select), M(cwk_gdn_scan), {NULL, NULL, 0, NULL}};
+    M(cwk_mla_decode), M(cwk_gqa_decode), M(cwk_dsa_select), M(cwk_gdn_scan), M(cwk_kv8_store), M(cwk_kv8_load),
+    M(cwk_gqa_qk_prep_kv8), M(cwk_gqa_decode_kv8), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__pycall(void) { return PyModule_Create(&module); }

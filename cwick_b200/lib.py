@@ -67,6 +67,11 @@ SIGNATURES = {
     "cwk_mm_index_scores": (i32, [vp, vp, i64, i32, vp, i32, vp]),
     "cwk_mm_select_blocks": (i32, [vp, vp, i64, i32, i32, i32, vp, vp, vp, vp]),
     "cwk_gqa_decode_sel": (i32, [vp, vp, vp, vp, i64, vp, i32, vp, i64, i32, i32, i32, i32, f32, vp, i32]),
+    "cwk_kv8_store": (i32, [vp, vp, vp, vp, i32, vp, vp, i32, i32]),
+    "cwk_kv8_load": (i32, [vp, vp, vp, vp, i32, i32, vp, vp, i32]),
+    "cwk_gqa_qk_prep_kv8": (i32, [vp] * 6 + [f32, i32, C.c_double, vp, vp, i32, i32, i32, vp, vp]),
+    "cwk_gqa_decode_kv8": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, f32, vp, i32]),
+    "cwk_gqa_prefill_kv8": (i32, [vp, vp, vp, i32, i64, i32, i32, f32, vp]),
     "cwk_kda_step": (i32, [vp, i32, i32, i32, f32, f32] + [vp] * 15),
     "cwk_ds_pool_norm": (i32, [vp, vp, vp, i32, i32, i32, vp, f32, vp]),
     "cwk_ds_rmsnorm_bf16w": (i32, [vp, vp, vp, i32, i32, f32, vp]),
@@ -78,6 +83,14 @@ SIGNATURES = {
     "cwk_mla_prefill": (i32, [vp] * 12 + [i64] + [i32] * 7 + [f32, f32, f32, vp]),
     "cwk_fp8_linear": (i32, [vp, vp, vp, vp, i64, i64, i64, vp, i32]),
 }
+
+class Kv8(C.Structure):
+    """cwk_kv8: a GQA cache held in 8 bits."""
+    _fields_ = [("k", vp), ("v", vp), ("k_scale", vp), ("v_scale", vp), ("rows", i64), ("slots", i32), ("nkv", i32), ("hd", i32), ("block", i32),
+                ("type", i32)]
+
+
+KV8_E4M3, KV8_INT8 = 0, 1
 
 # reference-named entry points (include/cwick_compat.h); bound separately because their
 # arguments are the reference's structs

@@ -20,6 +20,38 @@ def _bf16(t):
     return t
 
 
+def _i32(t, B):
+    """The address of an int32 [B] cuda tensor, or None."""
+    if t is None:
+        return None
+    assert t.dtype == torch.int32 and t.is_cuda and t.is_contiguous() and t.shape == (B,)
+    return t.data_ptr()
+
+
+class Kv8Cache:
+    """A GQA cache held in 8 bits (cwk_kv8): codes uint8 [slots][rows][nkv][hd] and scale bytes uint8 [slots][rows / block][nkv] for K and V, on
+    tensors of the caller's. `type`: "e4m3" or "int8"."""
+    TYPES = {"e4m3": _lib.KV8_E4M3, "int8": _lib.KV8_INT8}
+
+    def __init__(self, k, v, k_scale, v_scale, block=64, type="e4m3"):
+        slots, rows, nkv, hd = k.shape
+        for t in (k, v):
+            assert t.dtype == torch.uint8 and t.is_cuda and t.is_contiguous() and t.shape == k.shape and t.device == k.device
+        for t in (k_scale, v_scale):
+            assert t.dtype == torch.uint8 and t.is_contiguous() and t.shape == (slots, rows // block, nkv) and t.device == k.device
+        self.k, self.v, self.k_scale, self.v_scale, self.block, self.type = k, v, k_scale, v_scale, block, type
+        self.slots, self.rows, self.nkv, self.hd = slots, rows, nkv, hd
+        self.c = _lib.Kv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), rows, slots, nkv, hd, block, self.TYPES[type])
+        self.address = _lib.C.addressof(self.c)
+
+    @classmethod
+    def empty(cls, slots, rows, nkv, hd, block=64, type="e4m3", device="cuda"):
+        """Room for `rows` rows (a multiple of `block`) in each of `slots` slots."""
+        k, v = (torch.empty(slots, rows, nkv, hd, dtype=torch.uint8, device=device) for _ in range(2))
+        ks, vs = (torch.empty(slots, rows // block, nkv, dtype=torch.uint8, device=device) for _ in range(2))
+        return cls(k, v, ks, vs, block, type)
+
+
 class Attn:
     def __init__(self, device=0):
         torch.cuda.set_device(device)
@@ -29,6 +61,8 @@ class Attn:
         # the calls of a decode step: plain integers and floats in, status out
         self._mla_decode, self._gqa_decode, self._dsa_select, self._gdn_scan = (
             _lib.fast(self.lib, "cwk_" + n) for n in ("mla_decode", "gqa_decode", "dsa_select", "gdn_scan"))
+        self._kv8_store, self._kv8_load, self._gqa_qk_prep_kv8, self._gqa_decode_kv8 = (
+            _lib.fast(self.lib, "cwk_" + n) for n in ("kv8_store", "kv8_load", "gqa_qk_prep_kv8", "gqa_decode_kv8"))
 
     # ---- MLA ---------------------------------------------------------------
     def mla_decode(self, q, cache, kv_len, max_kv_len=None, sel=None, scale=None, seq_stride=None,
@@ -167,6 +201,74 @@ class Attn:
         out = torch.empty(n, nh, hd, dtype=torch.bfloat16, device=Q.device)
         self.ctx.check(self.lib.cwk_gqa_prefill(self.ctx.h, _p(Q), _p(K), _p(V), pos, n, nh, nkv, hd, scale,
                                                 _p(out)))
+        return out
+
+    # ---- GQA cache held in 8 bits ----------------------------------------------------
+    def kv8_store(self, cache, k, v, pos, count=None):
+        """Rows pos[b] .. of slot b from k, v [B][n][nkv][hd] (bf16 or f32); pos, count int32 [B] cuda (count None: n rows each)."""
+        B, n = k.shape[:2]
+        assert k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.is_contiguous() and v.is_contiguous()
+        assert k.shape == v.shape == (B, n, cache.nkv, cache.hd)
+        st = self._kv8_store(self.ctx.address, cache.address, k.data_ptr(), v.data_ptr(), 1 if k.dtype == torch.float32 else 0,
+                             _i32(pos, B), _i32(count, B), B, n)
+        if st:
+            self.ctx.check(st)
+
+    def kv8_load(self, cache, pos, n, count=None, dtype=torch.bfloat16, out=None):
+        """Rows pos[b] + 0 .. n - 1 of slot b as values: (K, V), each [B][n][nkv][hd]; rows from count[b] on are not written."""
+        B = pos.shape[0]
+        if out is None:
+            out = tuple(torch.empty(B, n, cache.nkv, cache.hd, dtype=dtype, device=cache.k.device) for _ in range(2))
+        k, v = out
+        assert k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.is_contiguous() and v.is_contiguous()
+        assert k.shape == v.shape == (B, n, cache.nkv, cache.hd)
+        st = self._kv8_load(self.ctx.address, cache.address, _i32(pos, B), _i32(count, B), B, n, k.data_ptr(), v.data_ptr(),
+                            1 if k.dtype == torch.float32 else 0)
+        if st:
+            self.ctx.check(st)
+        return k, v
+
+    def gqa_qk_prep_kv8(self, cache, qg, k, v, q_norm, k_norm, eps, rot, theta, pos, count=None, q_out=None):
+        """Norms, rotation and the cache's new rows in one pass (cwk_gqa_qk_prep_kv8): qg f32 [B][n][nh][2*hd], k, v f32 [B][n][nkv][hd].
+        Returns q bf16 [B][n][nh][hd]; rows from count[b] on are not written."""
+        B, n, nh, _ = qg.shape
+        for t in (qg, k, v, q_norm, k_norm):
+            assert t.dtype == torch.float32 and t.is_contiguous()
+        assert qg.shape[3] == 2 * cache.hd and k.shape == v.shape == (B, n, cache.nkv, cache.hd) and q_norm.numel() == k_norm.numel() == cache.hd
+        if q_out is None:
+            q_out = torch.empty(B, n, nh, cache.hd, dtype=torch.bfloat16, device=qg.device)
+        assert _bf16(q_out).shape == (B, n, nh, cache.hd)
+        st = self._gqa_qk_prep_kv8(self.ctx.address, qg.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), eps, rot,
+                                   theta, _i32(pos, B), _i32(count, B), B, n, nh, q_out.data_ptr(), cache.address)
+        if st:
+            self.ctx.check(st)
+        return q_out
+
+    def gqa_decode_kv8(self, q, cache, kv_len, scale=None, max_kv_len=None, n_splits=0, out=None):
+        """q bf16 [B][nh][hd], or [B][n][nh][hd] for n query tokens per sequence; kv_len int32 [B], those tokens' rows included."""
+        _bf16(q)
+        B, n, nh, hd = q.shape if q.dim() == 4 else (q.shape[0], 1, *q.shape[1:])
+        assert hd == cache.hd
+        if scale is None:
+            scale = 1.0 / math.sqrt(hd)
+        if max_kv_len is None:
+            max_kv_len = int(kv_len.max().item())
+        if out is None:
+            out = torch.empty_like(q)
+        assert _bf16(out).shape == q.shape
+        st = self._gqa_decode_kv8(self.ctx.address, q.data_ptr(), cache.address, _i32(kv_len, B), max_kv_len, B, n, nh, scale, out.data_ptr(), n_splits)
+        if st:
+            self.ctx.check(st)
+        return out
+
+    def gqa_prefill_kv8(self, Q, cache, pos, slot=0, scale=None):
+        """Q bf16 [n][nh][hd] at positions pos .. of a slot, whose rows up to pos + n are in the cache."""
+        _bf16(Q)
+        n, nh, hd = Q.shape
+        assert hd == cache.hd
+        out = torch.empty_like(Q)
+        self.ctx.check(self.lib.cwk_gqa_prefill_kv8(self.ctx.h, _p(Q), cache.address, slot, pos, n, nh, 1.0 / math.sqrt(hd) if scale is None else scale,
+                                                    _p(out)))
         return out
 
     # ---- FP8 projection ------------------------------------------------------------

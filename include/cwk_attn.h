@@ -13,7 +13,7 @@
  *   latent cache   bf16 [rows][ld]          row = [L latent | R rope key], ld >= L+R
  *   MLA query      bf16 [B][nh][L+R]        q_nope already absorbed through W_k
  *   MLA output     bf16 [B][nh][L]          softmax-weighted latent
- *   GQA cache      bf16 [rows][nkv][hd]     K and V separate
+ *   GQA cache      bf16 [rows][nkv][hd]     K and V separate (in 8 bits: cwk_kv8)
  *   partial        f32  {m[nh], l[nh], o[nh][L]}  l = sum e^(s-m), o = sum e^(s-m) c, un-normalised;
  *                  m is a per-head reference exponent (close to, not always equal to, the
  *                  maximum score): only m + log(l) and o/l are meaningful on their own
@@ -272,6 +272,51 @@ CWK_API int cwk_gqa_decode_sel(cwk_ctx *ctx, const void *q, const void *K, const
  *   Q bf16 [n][nh][hd]; K,V bf16 [pos+n][nkv][hd]; out bf16 [n][nh][hd]. */
 CWK_API int cwk_gqa_prefill(cwk_ctx *ctx, const void *Q, const void *K, const void *V, int64_t pos,
                     int n, int nh, int nkv, int hd, float scale, void *out);
+
+/* ---- GQA cache held in 8 bits ------------------------------------------------
+ * No counterpart in the reference, whose GQA cache is bf16 (src/q35_model.c:1558-1575): half the bytes per cached row, so twice the
+ * context in the same memory and, where decode is bound by reading the cache, up to twice the tokens. A slot's rows are codes, E4M3
+ * or two's complement INT8, in the bf16 cache's order; every `block` consecutive rows (from row 0 on) of a KV head share one
+ * scale, for K and for V each, stored as a biased exponent byte s (E8M0, 1..254): value = code * 2^(s - 127). The values are exact in bf16.
+ * The caller owns all arrays (device memory, codes 16-byte aligned); they need no initialisation. */
+enum { CWK_KV8_E4M3 = 0, CWK_KV8_INT8 = 1 };
+typedef struct cwk_kv8 {
+    void *k, *v;                  /* codes, one byte each: [slots][rows][nkv][hd] */
+    uint8_t *k_scale, *v_scale;   /* [slots][rows / block][nkv] */
+    int64_t rows;                 /* rows of a slot, a multiple of block */
+    int slots, nkv, hd;           /* hd 128 or 256 */
+    int block;                    /* 32, 64 or 128 */
+    int type;                     /* CWK_KV8_E4M3 or CWK_KV8_INT8 */
+} cwk_kv8;
+
+/* Rows pos[b] .. pos[b] + count[b] - 1 of slots b = 0 .. B - 1 from k, v [B][n][nkv][hd], bf16 or (f32 != 0) f32; pos, count int32
+ * [B] on the device, count NULL: n each, otherwise at most n (what is more is not read). Rows outside the slot are left out.
+ * A block's exponent is the least e with |x| <= 448 * 2^e (E4M3; INT8: 127) for its finite new values, within [-100, 119]
+ * (INT8: 121); a block that begins before pos[b] is open: rows in front of pos[b] stay what they are, e is at least the block's old one, and where
+ * it grows their codes move to the new scale, rounded to nearest (E4M3: exact unless they become subnormal). code = x / 2^e to
+ * nearest, ties to even; what is larger, infinities too, saturates; NaN is E4M3's NaN in keys, 0 in values and in INT8. So the result does not depend on how
+ * the rows were dealt out to calls, but for the roundings of codes that moved. Rows behind the new ones are not touched: the
+ * scale of the last block is no longer theirs. */
+CWK_API int cwk_kv8_store(cwk_ctx *ctx, const cwk_kv8 *cache, const void *k, const void *v, int f32, const int32_t *pos, const int32_t *count,
+                          int B, int n);
+/* The other way: the values of rows pos[b] + j, j < count[b] (NULL: n), into k, v [B][n][nkv][hd], bf16 or (f32 != 0) f32, exactly. Rows
+ * outside the slot and rows from count[b] on are left as they were. */
+CWK_API int cwk_kv8_load(cwk_ctx *ctx, const cwk_kv8 *cache, const int32_t *pos, const int32_t *count, int B, int n, void *k, void *v, int f32);
+/* cwk_gqa_qk_prep for B slots at positions of their own and this cache: RMS norm with (1 + w) weights of query and key heads, rotate-half
+ * RoPE on the first `rot` values (a multiple of 16), queries to bf16, keys and values into the cache as cwk_kv8_store does. qg f32
+ * [B][n][nh][2*hd] (q | gate per head), k, v f32 [B][n][nkv][hd], q_norm, k_norm f32 [hd], q_out bf16 [B][n][nh][hd]. pos, count as above;
+ * the query rows of tokens from count[b] on are left as they were. Angles, and keys up to their code, are formed in double. */
+CWK_API int cwk_gqa_qk_prep_kv8(cwk_ctx *ctx, const float *qg, const float *k, const float *v, const float *q_norm, const float *k_norm, float eps,
+                                int rot, double theta, const int32_t *pos, const int32_t *count, int B, int n, int nh, void *q_out,
+                                const cwk_kv8 *cache);
+/* cwk_gqa_decode over this cache, for n >= 1 query tokens per sequence: the last n of the kv_len[b] rows are those of the query tokens, token
+ * i sees rows 0 .. kv_len[b] - n + i (none: zeros). q, out bf16 [B][n][nh][hd], sequence b in slot b, kv_len int32 [B] device, at most max_kv_len
+ * (a larger one counts as the slot's rows), nh / nkv at most 16. Up to 16 / (nh / nkv) tokens share a pass over the cache. */
+CWK_API int cwk_gqa_decode_kv8(cwk_ctx *ctx, const void *q, const cwk_kv8 *cache, const int32_t *kv_len, int max_kv_len, int B, int n, int nh,
+                               float scale, void *out, int n_splits);
+/* cwk_gqa_prefill over this cache: queries at positions pos .. pos + n - 1 of one slot against its first pos + n rows.
+ * Q, out bf16 [n][nh][hd]; nh / nkv 1, 2, 4, 8 or 16. Workspace inside the context: 4 bytes per cached value. */
+CWK_API int cwk_gqa_prefill_kv8(cwk_ctx *ctx, const void *Q, const cwk_kv8 *cache, int slot, int64_t pos, int n, int nh, float scale, void *out);
 
 /* ---- FP8 block-scaled projection -------------------------------------------
  * Y[n][cols] = X[n][k] . W[cols][k]^T with W in E4M3 and one F32 multiplier
