@@ -41,22 +41,30 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_16816_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {      // the first of a sum
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-template <int HD> constexpr int KV8_STAGES = HD == 256 ? 3 : 6;
+// Places of a warp's ring, each the K or the V of a step: 24 KB a warp, so that two blocks of four warps are on an SM and a scheduler has
+// two of these chains of dependent instructions to choose from.
+template <int HD> constexpr int KV8_RING = HD == 256 ? 3 : 6;
 
 // NB: groups of eight MMA columns (query rows)
 template <int HD, int NB, bool I8>
-__global__ void __launch_bounds__(32 * GW) kv8_decode_kernel(const Kv8DecodeParams p) {
+__global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeParams p) {
     constexpr int CH = HD / 16;                           // 16-byte pieces per row
-    constexpr int STAGES = KV8_STAGES<HD>;
-    constexpr int KB = GK * HD;                           // bytes of a stage's K (and of its V)
+    constexpr int RING = KV8_RING<HD>;
+    constexpr int KB = GK * HD;                           // bytes of a place of the ring
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
-    const uint32_t ring = smem_u32(smem) + warp * STAGES * 2 * KB;
+    const uint32_t ring = smem_u32(smem) + warp * RING * KB;
     const int sub = warp / p.hb, wh = warp % p.hb;        // which 32 keys of a step, which KV head of the group
     const int keys = p.steps.keys, cols = p.per * p.group;
     GqaPlace at{0, 0, 0, 0, 0};
@@ -67,21 +75,26 @@ __global__ void __launch_bounds__(32 * GW) kv8_decode_kernel(const Kv8DecodePara
     at.len = length_of(p.steps, at.b);
     GqaPlace ld = at;                                     // the step being loaded
     auto head_of = [&](const GqaPlace &x) { return (x.hg / p.parts) * p.hb + wh; };
-    auto load = [&](int slot) {
-        const int j0 = ld.step * keys + sub * GK;
-        const int64_t row = (int64_t)p.nkv * HD, base = (int64_t)ld.b * p.rows * row + head_of(ld) * HD;
-        const uint32_t dst = ring + slot * 2 * KB;
-        constexpr int RPI = 32 / CH;                      // rows per instruction: 2 or 4
-        const int c = lane % CH, rr = lane / CH;
+    int halves = 2 * n, ld_place = 0;                     // halves of steps (K, then V) still to be asked for; the place of the next one
+    auto load_next = [&]() {
+        if (halves > 0) {
+            const int j0 = ld.step * keys + sub * GK;
+            const int64_t row = (int64_t)p.nkv * HD;
+            const uint8_t *src = ((halves & 1) ? p.v : p.k) + (int64_t)ld.b * p.rows * row + head_of(ld) * HD;
+            const uint32_t dst = ring + ld_place * KB;
+            constexpr int RPI = 32 / CH;                  // rows per instruction: 2 or 4
+            const int c = lane % CH, rr = lane / CH;
 #pragma unroll
-        for (int i = 0; i < GK / RPI; i++) {
-            const int r = i * RPI + rr;
-            const bool ok = j0 + r < ld.len;              // (rows behind the last are not read: zeros in their place)
-            const int64_t off = base + (ok ? (int64_t)(j0 + r) * row : 0) + c * 16;
-            const uint32_t d = dst + r * HD + ((c ^ (r & 7)) << 4);
-            cp_async16(d, p.k + off, ok);
-            cp_async16(d + KB, p.v + off, ok);
+            for (int i = 0; i < GK / RPI; i++) {
+                const int r = i * RPI + rr;
+                const bool ok = j0 + r < ld.len;          // (rows behind the last are not read: zeros in their place)
+                cp_async16(dst + r * HD + ((c ^ (r & 7)) << 4), src + (ok ? (int64_t)(j0 + r) * row : 0) + c * 16, ok);
+            }
+            halves--;
+            ld_place = ld_place + 1 == RING ? 0 : ld_place + 1;
+            if (halves > 0 && !(halves & 1)) gqa_advance(p.steps, ld);
         }
+        cp_async_commit();
     };
     // the two scales of this warp's keys at a place (any value where it has no key there)
     auto scales = [&](const GqaPlace &x) -> uint32_t {
@@ -90,19 +103,15 @@ __global__ void __launch_bounds__(32 * GW) kv8_decode_kernel(const Kv8DecodePara
         const int64_t i = ((int64_t)x.b * (p.rows >> p.lb) + (j0 >> p.lb)) * p.nkv + head_of(x);
         return (uint32_t)p.ks[i] | (uint32_t)p.vs[i] << 8;
     };
-    for (int s = 0; s < STAGES - 1; s++) {
-        if (s < n) {
-            load(s);
-            if (s + 1 < n) gqa_advance(p.steps, ld);
-        }
-        cp_async_commit();
-    }
+#pragma unroll
+    for (int i = 0; i < RING - 1; i++) load_next();
     uint32_t bq[HD / 16][NB][2];                          // the query rows, as the score MMAs' second operand
     float acc[HD / 16][NB][4];                            // value columns 16 i + 2 lg (+ 1) of query rows 8 nb + 2 lt, + 1
     float m[NB][2], l[NB][2], unit[NB][2];                // unit: what a score MMA's result is multiplied by, besides the key scale
     int limit[NB][2];                                     // rows that the query row sees
     uint32_t sc = scales(at);
     bool fresh = true;
+    int place = 0;                                        // of the half in use
     for (int s = 0; s < n; s++) {
         if (fresh) {
             const int part = at.hg % p.parts;
@@ -140,27 +149,20 @@ __global__ void __launch_bounds__(32 * GW) kv8_decode_kernel(const Kv8DecodePara
                 }
             }
         }
-        cp_async_wait<STAGES - 2>();
-        __syncwarp();                                     // every lane's copies of this step have landed; the last step's slot has been read
-        if (s + STAGES - 1 < n) {
-            load((s + STAGES - 1) % STAGES);
-            if (s + STAGES < n) gqa_advance(p.steps, ld);
-        }
-        cp_async_commit();
+        cp_async_wait<RING - 2>();
+        __syncwarp();                                     // every lane's copies of these keys have landed; the place before has been read
+        load_next();
         GqaPlace next = at;                               // its scales are asked for a step ahead
         uint32_t sc_next = 0;
         if (s + 1 < n) {
             gqa_advance(p.steps, next);
             sc_next = scales(next);
         }
-        const uint32_t tK = ring + (s % STAGES) * 2 * KB, tV = tK + KB;
+        const uint32_t tK = ring + place * KB;
+        place = place + 1 == RING ? 0 : place + 1;
         const uint32_t row = lane * HD, x7 = lane & 7;    // ldmatrix: a lane's address is key `lane`'s
         const float kscale = kv8_scale(sc & 255u), vscale = kv8_scale(sc >> 8);
         float c[2][NB][4];                                // scores of keys 16 h + lg, + 8
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) c[h][nb][0] = c[h][nb][1] = c[h][nb][2] = c[h][nb][3] = 0.f;
 #pragma unroll
         for (int i = 0; i < HD / 16; i++) {
             uint32_t r[4], a[2][4];
@@ -170,7 +172,10 @@ __global__ void __launch_bounds__(32 * GW) kv8_decode_kernel(const Kv8DecodePara
                 kv8_decode4<I8>(r[2 * h], a[h][0], a[h][2]);
                 kv8_decode4<I8>(r[2 * h + 1], a[h][1], a[h][3]);
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++) mma_f16_16816(c[h][nb], a[h], bq[i][nb][0], bq[i][nb][1]);
+                for (int nb = 0; nb < NB; nb++) {
+                    if (i == 0) mma_f16_16816_zero(c[h][nb], a[h], bq[i][nb][0], bq[i][nb][1]);
+                    else mma_f16_16816(c[h][nb], a[h], bq[i][nb][0], bq[i][nb][1]);
+                }
             }
         }
         const int j0 = at.step * keys + sub * GK + lg;    // this lane's keys: j0, + 8, + 16, + 24
@@ -220,19 +225,25 @@ __global__ void __launch_bounds__(32 * GW) kv8_decode_kernel(const Kv8DecodePara
                 asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(w));
             }
         }
+        cp_async_wait<RING - 2>();                        // the same for the values
+        __syncwarp();
+        load_next();
+        const uint32_t tV = ring + place * KB;
+        place = place + 1 == RING ? 0 : place + 1;
 #pragma unroll
         for (int i = 0; i < HD / 16; i++) {
             uint32_t r[4], a[2][4];
             ldmatrix_x4_trans(r[0], r[1], r[2], r[3], tV + row + ((i ^ x7) << 4));
             float d[NB][4];
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++) d[nb][0] = d[nb][1] = d[nb][2] = d[nb][3] = 0.f;
-#pragma unroll
             for (int h = 0; h < 2; h++) {
                 kv8_decode4_even_odd<I8>(r[2 * h], a[h][0], a[h][1]);
                 kv8_decode4_even_odd<I8>(r[2 * h + 1], a[h][2], a[h][3]);
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++) mma_f16_16816(d[nb], a[h], b[h][nb][0], b[h][nb][1]);
+                for (int nb = 0; nb < NB; nb++) {
+                    if (h == 0) mma_f16_16816_zero(d[nb], a[h], b[h][nb][0], b[h][nb][1]);
+                    else mma_f16_16816(d[nb], a[h], b[h][nb][0], b[h][nb][1]);
+                }
             }
 #pragma unroll
             for (int nb = 0; nb < NB; nb++)
@@ -285,7 +296,7 @@ __global__ void __launch_bounds__(HD / 2 * GROUPS) kv8_merge_kernel(const Kv8Dec
 
 template <int HD, int NB>
 int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *out) {
-    constexpr int SMEM = GW * KV8_STAGES<HD> * 2 * GK * HD;      // 192 KB
+    constexpr int SMEM = GW * KV8_RING<HD> * GK * HD;      // 96 KB
     const bool i8 = type == CWK_KV8_INT8;
     auto kern = i8 ? kv8_decode_kernel<HD, NB, true> : kv8_decode_kernel<HD, NB, false>;
     static bool attr_set[2][16] = {};
@@ -316,11 +327,11 @@ int cwk_kv8_streams(cwk_ctx *ctx, const void *q, const cwk_kv8 &c, const int32_t
     p.per = std::min(n, std::max(1, 16 / p.group));
     p.parts = (n + p.per - 1) / p.per;
     p.scale_log2 = scale * 1.4426950408889634f;
-    // as many blocks as there can be steps, at most one per SM
+    // as many blocks as there can be steps, at most two per SM
     const int keys = GK * (GW / p.hb);
     const int64_t groups = (int64_t)(c.nkv / p.hb) * p.parts;
     const int64_t most = std::max<int64_t>(1, B * groups * ((max_kv_len + keys - 1) / keys));
-    const int blocks = (int)std::min<int64_t>(most, max_blocks > 0 ? std::min(max_blocks, ctx->sm_count) : ctx->sm_count);
+    const int blocks = (int)std::min<int64_t>(most, max_blocks > 0 ? std::min(max_blocks, 2 * ctx->sm_count) : 2 * ctx->sm_count);
     const size_t rec_bytes = (size_t)(B * groups + blocks) * GW * p.per * p.group * (c.hd + 2) * sizeof(float);
     const int s = cwk_reserve_scratch(ctx, rec_bytes + (size_t)B * groups * sizeof(int2));
     if (s != CWK_OK) return s;
