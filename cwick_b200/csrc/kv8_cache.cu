@@ -1,8 +1,8 @@
 // kv8_cache.cu -- writing and reading the GQA cache held in 8 bits (format: kv8.cuh), compiled without fast-math.
 //
-// Writing. A task is one block of rows of one KV head, K or V: its new rows are read once into registers (a warp has up to eight of them, a
-// lane hd / 32 neighbouring values of each), the largest magnitude is found over the task, then the codes go out; an open block whose
-// scale grows has the codes in front of the new rows rewritten. In front of the quantisation, for cwk_gqa_qk_prep_kv8, keys get
+// Writing. A task is one block of rows of one KV head, K or V: its new rows are read once into registers (a warp has four or eight rows in a
+// row, a lane hd / 32 neighbouring values of each), the largest magnitude is found over the task, then the codes go out; an open block
+// whose scale grows has the codes in front of the new rows rewritten. In front of the quantisation, for cwk_gqa_qk_prep_kv8, keys get
 // their RMS norm and rotation (src/q35_model.c:112-122, :144-153, :459-477), and query heads the same on blocks of their own.
 #include <algorithm>
 #include <cmath>
@@ -10,8 +10,6 @@
 #include "kv8.cuh"
 
 namespace {
-
-constexpr int KW_ROWS = 8;                     // rows per warp
 
 enum { SRC_BF16 = 0, SRC_F32 = 1 };
 
@@ -29,8 +27,10 @@ struct Kv8WriteParams {
     float eps;
     int64_t tasks;                             // K and V tasks; the blocks behind them have query rows
     int heads;                                 // query heads per warp
-    double inv_freq[128];
+    double freq[128];                          // angle of a pair per position
+    double2 turn[128];                         // its cos and sin
 };
+constexpr int KQ_HEADS = 4;                    // most query heads of a warp
 
 // new rows of slot b: positions pos .. pos + the result - 1, all inside the slot
 __device__ __forceinline__ int new_rows(const Kv8WriteParams &p, int b, int64_t &pos) {
@@ -39,53 +39,64 @@ __device__ __forceinline__ int new_rows(const Kv8WriteParams &p, int b, int64_t 
     return pos < 0 ? 0 : (int)max((int64_t)0, min(c, p.rows - pos));
 }
 
+// A lane's V values of a row, as they lie in memory (two bf16 or one f32 a word).
 template <int V, int SRC>
-__device__ __forceinline__ void load_row(const void *src, int64_t row, int lane, float (&x)[V]) {
-    if constexpr (SRC == SRC_BF16) {
-        const uint16_t *s = (const uint16_t *)src + row * (32 * V) + lane * V;
-        if constexpr (V == 8) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(s);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct Raw {
+    static constexpr int W = SRC == SRC_BF16 ? V / 2 : V;
+    uint32_t w[W];
+    __device__ __forceinline__ void load(const void *src, int64_t row, int lane) {
+        const uint32_t *s = (const uint32_t *)src + (row * 32 + lane) * W;
+        if constexpr (W == 2) { const uint2 u = *reinterpret_cast<const uint2 *>(s); w[0] = u.x; w[1] = u.y; }
+        else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
-        } else {
-            const uint2 u = *reinterpret_cast<const uint2 *>(s);
-            const uint32_t w[2] = {u.x, u.y};
-#pragma unroll
-            for (int i = 0; i < 2; i++) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u); }
-        }
-    } else {
-        const float4 *s = reinterpret_cast<const float4 *>((const float *)src + row * (32 * V) + lane * V);
-#pragma unroll
-        for (int i = 0; i < V / 4; i++) {
-            const float4 f = s[i];
-            x[4 * i] = f.x; x[4 * i + 1] = f.y; x[4 * i + 2] = f.z; x[4 * i + 3] = f.w;
+            for (int i = 0; i < W / 4; i++) {
+                const uint4 u = reinterpret_cast<const uint4 *>(s)[i];
+                w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+            }
         }
     }
-}
-
-// finite magnitudes only: an infinity saturates and does not set the scale
-__device__ __forceinline__ float magnitude(float x) {
-    const float a = fabsf(x);
-    return a <= 3.4028235e38f ? a : 0.f;       // (false for NaN too)
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (SRC == SRC_BF16) return __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+        else return __uint_as_float(w[i]);
+    }
+    // bits of the largest magnitude; 0x7F800000 and up: there is a value that is not finite
+    __device__ __forceinline__ uint32_t magnitude() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < V; i++) m = max(m, __float_as_uint((*this)[i]) & 0x7FFFFFFFu);
+        return m;
+    }
+};
+__device__ __forceinline__ uint32_t finite_magnitude(float x) {
+    const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
+    return u < 0x7F800000u ? u : 0u;
 }
 
 // cos and sin of a position's angles, for the rot / 2 pairs of a head, by a warp into its share of shared memory
-__device__ __forceinline__ void angles(const Kv8WriteParams &p, int64_t pos, int lane, double2 *cs) {
-    for (int i = lane; i < p.rot / 2; i += 32) {
+__device__ __forceinline__ void angles(const double *freq, int pairs, int64_t pos, int lane, double2 *cs) {
+    for (int i = lane; i < pairs; i += 32) {
         double c, s;
-        sincos((double)pos * p.inv_freq[i], &s, &c);
+        sincos((double)pos * freq[i], &s, &c);
         cs[i] = make_double2(c, s);
+    }
+    __syncwarp();
+}
+// ... and of the next position: a turn by the angle of one. (At most seven in a row: an error of some 2^-50.)
+__device__ __forceinline__ void next_angles(const double2 *turn, int pairs, int lane, double2 *cs) {
+    __syncwarp();
+    for (int i = lane; i < pairs; i += 32) {
+        const double2 a = cs[i], b = turn[i];
+        cs[i] = make_double2(a.x * b.x - a.y * b.y, a.y * b.x + a.x * b.y);
     }
     __syncwarp();
 }
 
 // A row's norm and rotation by a warp: y = x * rstd * (1 + w), the first `rot` values turned in pairs (i, i + rot / 2). Keys in T = double:
 // a code hangs on which side of a border a value is, and this way it is the definition's; queries, which are rounded to bf16, in float.
-template <int V, class T>
-__device__ __forceinline__ void norm_rotate(const float (&x)[V], T rstd, const float (&w)[V], int rot, int lane, const double2 *cs, T (&y)[V]) {
+template <int V, class T, class X>
+__device__ __forceinline__ void norm_rotate(const X &x, T rstd, const T (&w1)[V], int rot, int lane, const double2 *cs, T (&y)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; i++) y[i] = (T)x[i] * rstd * ((T)1 + (T)w[i]);
+    for (int i = 0; i < V; i++) y[i] = (T)x[i] * rstd * w1[i];
     if (rot == 0) return;
     const int d0 = lane * V, shift = rot / 2 / V;
     const bool lo = d0 < rot / 2, hi = !lo && d0 < rot;
@@ -95,13 +106,13 @@ __device__ __forceinline__ void norm_rotate(const float (&x)[V], T rstd, const f
         const T other = __shfl_sync(0xffffffffu, y[i], from);
         if (lo || hi) {
             const double2 t = cs[pair + i];
-            const T c = (T)t.x, s = (T)t.y;
-            y[i] = lo ? y[i] * c - other * s : y[i] * c + other * s;
+            const T c = (T)t.x, s = lo ? -(T)t.y : (T)t.y;
+            y[i] = y[i] * c + other * s;
         }
     }
 }
-template <int V, class T>
-__device__ __forceinline__ T row_rstd(const float (&x)[V], float eps) {
+template <int V, class T, class X>
+__device__ __forceinline__ T row_rstd(const X &x, float eps) {
     T sum = 0;
 #pragma unroll
     for (int i = 0; i < V; i++) sum += (T)x[i] * (T)x[i];
@@ -110,31 +121,40 @@ __device__ __forceinline__ T row_rstd(const float (&x)[V], float eps) {
     return (T)1 / sqrt(sum / (T)(32 * V) + (T)eps);
 }
 
-// double -> float for a second rounding to few bits: towards zero, the last bit set where anything was cut off, so that the
-// second rounding sees on which side of a tie the value is
+// double -> float for a second rounding to few bits: cut off, the last bit set where anything was, so that the second rounding sees
+// on which side of a tie the value is. Integer work (conversions run at a quarter of its rate); below 2^-126 it is zero.
 __device__ __forceinline__ float to_odd(double y) {
-    const float f = __double2float_rz(y);
-    return (double)f != y && y == y ? __uint_as_float(__float_as_uint(f) | 1u) : f;
+    const uint32_t hi = (uint32_t)__double2hiint(y), lo = (uint32_t)__double2loint(y), mag = hi & 0x7FFFFFFFu;
+    const uint32_t f = (mag - 0x38000000u) << 3 | lo >> 29 | (lo << 3 != 0u ? 1u : 0u);
+    return __uint_as_float((hi & 0x80000000u) | (mag < 0x38100000u ? 0u : mag >= 0x47F00000u ? (mag > 0x7FF00000u || (mag == 0x7FF00000u && lo) ? 0x7FC00000u : 0x7F800000u) : f));
 }
 
-template <int V, bool I8>
-__device__ __forceinline__ void store_codes(uint8_t *dst, const float (&y)[V]) {
-    uint32_t w[V / 4];
-#pragma unroll
-    for (int i = 0; i < V / 4; i++) {
-        const float t[4] = {y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
-        w[i] = kv8_encode4<I8>(t);
-    }
+template <int V>
+__device__ __forceinline__ void store_words(uint8_t *dst, const uint32_t (&w)[V / 4]) {
     if constexpr (V == 8) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t *>(dst) = w[0];
 }
-
-// A NaN among keys shows in the scores of the queries that see it. Among values it would reach queries that do not: their
-// probability of it is zero, but the product is not. So values take zero in its place.
-template <int V>
-__device__ __forceinline__ void no_nan(float (&y)[V]) {
+// Codes of values in units of the scale. careful: some are not finite, or larger than the largest code.
+template <int V, bool I8>
+__device__ __forceinline__ void store_codes(uint8_t *dst, const float (&y)[V], bool careful, bool is_v) {
+    uint32_t w[V / 4];
 #pragma unroll
-    for (int j = 0; j < V; j++) if (y[j] != y[j]) y[j] = 0.f;
+    for (int i = 0; i < V / 4; i++) {
+        float t[4] = {y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
+        if (careful) {
+            // A NaN among keys shows in the scores of the queries that see it. Among values it would reach queries that do not: their
+            // probability of it is zero, but the product is not. So values take zero in its place.
+#pragma unroll
+            for (int j = 0; j < 4; j++) if (is_v && t[j] != t[j]) t[j] = 0.f;
+            w[i] = kv8_encode4<I8>(t);
+        } else if constexpr (I8) {
+            uint32_t u[4];                     // plus 1.5 * 2^23: the nearest whole number (ties to even) in the low bits
+#pragma unroll
+            for (int j = 0; j < 4; j++) u[j] = __float_as_uint(t[j] + 12582912.f);
+            w[i] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+        } else w[i] = kv8_encode4<I8>(t);
+    }
+    store_words<V>(dst, w);
 }
 
 // Rows r0 .. r0 + lead - 1 of an open block move from scale 2^was to 2^e, e > was.
@@ -151,46 +171,59 @@ __device__ __forceinline__ void rescale(uint8_t *codes, int64_t ld, int lead, in
             const float2 u = __half22float2(*reinterpret_cast<const __half2 *>(&a)), v = __half22float2(*reinterpret_cast<const __half2 *>(&b));
             y[4 * i] = u.x * f; y[4 * i + 1] = u.y * f; y[4 * i + 2] = v.x * f; y[4 * i + 3] = v.y * f;
         }
-        if (is_v) no_nan(y);
-        store_codes<V, I8>(at, y);
+        store_codes<V, I8>(at, y, true, is_v);
     }
 }
 
-// V: values of a row per lane (head dim / 32). PREP: f32 rows, keys normed and rotated; blocks from p.tasks on have query rows.
-template <int V, int SRC, bool I8, bool PREP>
+// V: values of a row per lane (head dim / 32); ROWS: rows of a warp. PREP: f32 rows, keys normed and rotated; blocks from p.tasks on have
+// query rows.
+template <int V, int SRC, bool I8, bool PREP, int ROWS>
 __global__ void __launch_bounds__(512) kv8_write_kernel(const __grid_constant__ Kv8WriteParams p) {
     constexpr int HD = 32 * V;
-    extern __shared__ double2 s_cs[];                      // PREP: [warp][rot / 2]
-    __shared__ float s_max[16];
+    extern __shared__ double2 s_dyn[];                     // PREP: [warp][rot / 2] cos and sin, [rot / 2] turns, [rot / 2] frequencies
+    __shared__ uint32_t s_max[16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int pairs = p.rot / 2;
+    double2 *cs = s_dyn + warp * pairs, *turn = s_dyn + warps * pairs;
+    double *freq = reinterpret_cast<double *>(turn + pairs);
     cwk_pdl_launch();
+    if (PREP) {
+        for (int i = threadIdx.x; i < pairs; i += blockDim.x) { turn[i] = p.turn[i]; freq[i] = p.freq[i]; }
+        __syncthreads();
+    }
     cwk_pdl_wait();
-    double2 *cs = s_cs + warp * (p.rot / 2);
     if (PREP && blockIdx.x >= p.tasks) {
         // ---- query rows: a warp has `heads` heads of one token
         const int parts = (p.nh + p.heads - 1) / p.heads;
         const int64_t id = ((int64_t)blockIdx.x - p.tasks) * warps + warp, t = id / parts;
         if (t >= (int64_t)p.B * p.n) return;
-        const int b = (int)(t / p.n), j = (int)(t % p.n), h0 = (int)(id % parts) * p.heads;
+        const int b = (int)(t / p.n), j = (int)(t % p.n), h0 = (int)(id % parts) * p.heads, mine = min(p.heads, p.nh - h0);
+        Raw<V, SRC_F32> x[KQ_HEADS], w;
+        w.load(p.q_norm, 0, lane);
+#pragma unroll
+        for (int i = 0; i < KQ_HEADS; i++)
+            if (i < mine) x[i].load(p.qg, (t * p.nh + h0 + i) * 2, lane);      // rows [q | gate] of 2 * hd
         int64_t pos;
         if (j >= new_rows(p, b, pos)) return;
-        angles(p, pos + j, lane, cs);
-        float w[V];
-        load_row<V, SRC_F32>(p.q_norm, 0, lane, w);
-        for (int h = h0; h < min(h0 + p.heads, p.nh); h++) {
-            float x[V], y[V];
-            load_row<V, SRC_F32>(p.qg, (t * p.nh + h) * 2, lane, x);      // rows [q | gate] of 2 * hd
-            norm_rotate<V, float>(x, row_rstd<V, float>(x, p.eps), w, p.rot, lane, cs, y);
+        angles(freq, pairs, pos + j, lane, cs);
+        float w1[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) w1[i] = 1.f + w[i];
+#pragma unroll
+        for (int i = 0; i < KQ_HEADS; i++) {
+            if (i >= mine) break;
+            float y[V];
+            norm_rotate<V, float>(x[i], row_rstd<V, float>(x[i], p.eps), w1, p.rot, lane, cs, y);
             uint32_t o[V / 2];
 #pragma unroll
-            for (int i = 0; i < V / 2; i++) o[i] = pack_bf16x2(y[2 * i], y[2 * i + 1]);
-            uint16_t *dst = p.q_out + (t * p.nh + h) * HD + lane * V;
+            for (int k = 0; k < V / 2; k++) o[k] = pack_bf16x2(y[2 * k], y[2 * k + 1]);
+            uint16_t *dst = p.q_out + (t * p.nh + h0 + i) * HD + lane * V;
             if constexpr (V == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
             else *reinterpret_cast<uint2 *>(dst) = make_uint2(o[0], o[1]);
         }
         return;
     }
-    int64_t id = blockIdx.x;
+    uint32_t id = blockIdx.x;
     const int head = (int)(id % p.nkv); id /= p.nkv;
     const int win = (int)(id % p.window); id /= p.window;
     const int b = (int)(id % p.B);
@@ -201,45 +234,64 @@ __global__ void __launch_bounds__(512) kv8_write_kernel(const __grid_constant__ 
     const int64_t lo = max(r0, pos), hi = min(r0 + (1 << p.lb), pos + cnt);
     if (lo >= hi) return;
     const bool norm = PREP && !is_v;
-    const void *src = is_v ? p.v : p.k;
     uint8_t *codes = (is_v ? p.vc : p.kc) + (((int64_t)b * p.rows + r0) * p.nkv + head) * HD;
     uint8_t *scale = (is_v ? p.vs : p.ks) + ((int64_t)b * (p.rows >> p.lb) + blk) * p.nkv + head;
     const int64_t ld = (int64_t)p.nkv * HD;
-    const int lead = (int)(lo - r0);
+    const int lead = (int)(lo - r0), many = (int)(hi - lo);
     const int was_byte = lead > 0 ? (int)*scale : 0;
-    float x[KW_ROWS][V], w[V];
-    double rstd[KW_ROWS];
-    float amax = 0.f;
-    // row i of this warp: lo + warp + i * warps
+    const int first = warp * ROWS;                         // this warp's rows: lo + first .. + ROWS - 1, those below hi
+    Raw<V, SRC> x[ROWS];
+    double w1[V], rstd[ROWS];
+    uint32_t amax = 0;
+    {
+        const void *src = is_v ? p.v : p.k;
+        const int64_t row = ((int64_t)b * p.n + (lo - pos) + first) * p.nkv + head;
 #pragma unroll
-    for (int i = 0; i < KW_ROWS; i++) {
-        const int64_t r = lo + warp + i * warps;
-        if (r < hi) load_row<V, SRC>(src, ((int64_t)b * p.n + (r - pos)) * p.nkv + head, lane, x[i]);
+        for (int i = 0; i < ROWS; i++)
+            if (first + i < many) x[i].load(src, row + i * p.nkv, lane);
     }
-    if (norm) load_row<V, SRC_F32>(p.k_norm, 0, lane, w);
+    if (norm) {
+        Raw<V, SRC_F32> w;
+        w.load(p.k_norm, 0, lane);
 #pragma unroll
-    for (int i = 0; i < KW_ROWS; i++) {
-        const int64_t r = lo + warp + i * warps;
-        if (r >= hi) continue;                             // (the same for the whole warp)
+        for (int i = 0; i < V; i++) w1[i] = 1.0 + (double)w[i];
+        if (first < many) angles(freq, pairs, lo + first, lane, cs);
+    }
+    uint32_t all = 0;                                      // as amax, of all values
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        if (first + i >= many) continue;                   // (the same for the whole warp)
         if (norm) {
             double y[V];
             rstd[i] = row_rstd<V, double>(x[i], p.eps);
-            angles(p, r, lane, cs);
-            norm_rotate<V, double>(x[i], rstd[i], w, p.rot, lane, cs, y);
+            if (i > 0) next_angles(turn, pairs, lane, cs);
+            norm_rotate<V, double>(x[i], rstd[i], w1, p.rot, lane, cs, y);
 #pragma unroll
-            for (int j = 0; j < V; j++) amax = fmaxf(amax, magnitude(__double2float_ru(fabs(y[j]))));      // rounded up: never below the value
-            __syncwarp();
-        } else {
+            for (int j = 0; j < V; j++) {
+                const float up = __double2float_ru(fabs(y[j]));      // never below the value
+                amax = max(amax, finite_magnitude(up));
+                all = max(all, __float_as_uint(up) & 0x7FFFFFFFu);
+            }
+        } else all = max(all, x[i].magnitude());
+    }
+    if (!norm) {
+        amax = all;
+        if (all >= 0x7F800000u) {                          // an infinity saturates and does not set the scale; nor does a NaN
+            amax = 0;
 #pragma unroll
-            for (int j = 0; j < V; j++) amax = fmaxf(amax, magnitude(x[i][j]));
+            for (int i = 0; i < ROWS; i++) {
+                if (first + i >= many) continue;
+#pragma unroll
+                for (int j = 0; j < V; j++) amax = max(amax, finite_magnitude(x[i][j]));
+            }
         }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    amax = __reduce_max_sync(0xffffffffu, amax);
     if (lane == 0) s_max[warp] = amax;
-    __syncthreads();
-    for (int i = 0; i < warps; i++) amax = fmaxf(amax, s_max[i]);
-    int e = kv8_exponent(amax, I8);
+    const bool odd = __syncthreads_or(all >= 0x7F800000u);
+    for (int i = 0; i < warps; i++) amax = max(amax, s_max[i]);
+    int e = kv8_exponent(__uint_as_float(amax), I8);
+    const bool careful = odd || e == kv8_high(I8);
     if (lead > 0) {
         const int was = min(max(was_byte - 127, KV8_LOW), kv8_high(I8));
         if (was >= e) e = was;
@@ -247,28 +299,28 @@ __global__ void __launch_bounds__(512) kv8_write_kernel(const __grid_constant__ 
     }
     if (threadIdx.x == 0) *scale = (uint8_t)(e + 127);
     const float f = kv8_two(-e);
+    uint8_t *dst = codes + (lead + first) * ld + lane * V;
+    if (norm && first < many) angles(freq, pairs, lo + first, lane, cs);
 #pragma unroll
-    for (int i = 0; i < KW_ROWS; i++) {
-        const int64_t r = lo + warp + i * warps;
-        if (r >= hi) continue;
+    for (int i = 0; i < ROWS; i++, dst += ld) {
+        if (first + i >= many) continue;
         float y[V];
         if (norm) {
             double z[V];
-            angles(p, r, lane, cs);
-            norm_rotate<V, double>(x[i], rstd[i], w, p.rot, lane, cs, z);
-            __syncwarp();
-            // INT8: one rounding of the double; E4M3: to odd, then to nearest
+            if (i > 0) next_angles(turn, pairs, lane, cs);
+            norm_rotate<V, double>(x[i], rstd[i], w1, p.rot, lane, cs, z);
+            // INT8: the nearest whole number, as a float; E4M3: to odd, then (in store_codes) to nearest
 #pragma unroll
-            for (int j = 0; j < V; j++) y[j] = I8 ? (float)rint(fmin(fmax(z[j] * (double)f, -127.0), 127.0)) : to_odd(z[j] * (double)f);
-            // (a NaN goes through fmin and fmax as -127 or 127)
-#pragma unroll
-            for (int j = 0; j < V; j++) if (z[j] != z[j]) y[j] = NAN;
+            for (int j = 0; j < V; j++) {
+                if constexpr (I8) y[j] = careful ? (z[j] == z[j] ? (float)rint(fmin(fmax(z[j] * (double)f, -127.0), 127.0)) : 0.f)
+                                                 : (float)__double2loint(z[j] * (double)f + 6755399441055744.0);      // (plus 1.5 * 2^52)
+                else y[j] = to_odd(z[j] * (double)f);
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < V; j++) y[j] = x[i][j] * f;
         }
-        if (is_v) no_nan(y);
-        store_codes<V, I8>(codes + (r - r0) * ld + lane * V, y);
+        store_codes<V, I8>(dst, y, careful, is_v);
     }
 }
 
@@ -281,59 +333,57 @@ struct Kv8ReadParams {
     int64_t n;
     void *k, *v;
 };
-constexpr int KR_THREADS = 256, KR_UNROLL = 4;
+constexpr int KR_THREADS = 256, KR_ROWS = 8;
 
+// A thread has eight codes (head, place in it) of every `step`-th row of a slot, KR_ROWS rows in flight. grid (chunks of rows, slot, K or V)
 template <int HD, bool I8, bool F32>
 __global__ void __launch_bounds__(KR_THREADS) kv8_read_kernel(const Kv8ReadParams p) {
-    constexpr int PER = 8, CH = HD / PER;                  // values per thread and piece; pieces per head row
+    constexpr int PER = 8, CH = HD / PER;                  // codes per thread and row; such pieces of a head
     cwk_pdl_launch();
+    const int b = blockIdx.y, pieces = p.nkv * CH;         // of a row
+    // rows that the block's threads have at once; a row wider than the block is done in parts
+    const int step = max(KR_THREADS / pieces, 1), r = (int)threadIdx.x / pieces, at0 = (int)threadIdx.x % pieces;
+    if (r >= step) return;
     cwk_pdl_wait();
-    const uint8_t *codes = blockIdx.y ? p.vc : p.kc, *scales = blockIdx.y ? p.vs : p.ks;
-    uint8_t *out = (uint8_t *)(blockIdx.y ? p.v : p.k);
-    const int64_t total = (int64_t)p.B * p.n * p.nkv * CH;
-    const int64_t first = (int64_t)blockIdx.x * (KR_THREADS * KR_UNROLL) + threadIdx.x;
-    uint2 c[KR_UNROLL];
-    uint32_t s[KR_UNROLL];
-    bool on[KR_UNROLL];
+    const uint8_t *codes = (blockIdx.z ? p.vc : p.kc) + (int64_t)b * p.rows * p.nkv * HD, *scales = (blockIdx.z ? p.vs : p.ks) + (int64_t)b * (p.rows >> p.lb) * p.nkv;
+    uint8_t *out = (uint8_t *)(blockIdx.z ? p.v : p.k) + (int64_t)b * p.n * p.nkv * HD * (F32 ? 4 : 2);
+    const int64_t pos = p.pos ? (int64_t)p.pos[b] : p.row0;
+    const int64_t end = min(min(p.n, p.count ? (int64_t)p.count[b] : p.n), p.rows - pos), j0 = (int64_t)blockIdx.x * (step * KR_ROWS) + r;
+    for (int at = at0; at < pieces; at += KR_THREADS) {
+        const int head = at / CH;
+        uint2 c[KR_ROWS];
+        uint32_t s[KR_ROWS];
 #pragma unroll
-    for (int u = 0; u < KR_UNROLL; u++) {
-        const int64_t id = first + u * KR_THREADS;
-        on[u] = id < total;
-        if (!on[u]) continue;
-        const int piece = (int)(id % CH);
-        const int64_t rh = id / CH;
-        const int head = (int)(rh % p.nkv);
-        const int64_t row = rh / p.nkv, j = row % p.n;
-        const int b = (int)(row / p.n);
-        const int64_t r = (p.pos ? (int64_t)p.pos[b] : p.row0) + j;
-        on[u] = r >= 0 && r < p.rows && (!p.count || j < p.count[b]);
-        if (!on[u]) continue;
-        c[u] = *reinterpret_cast<const uint2 *>(codes + (((int64_t)b * p.rows + r) * p.nkv + head) * HD + piece * PER);
-        s[u] = scales[((int64_t)b * (p.rows >> p.lb) + (r >> p.lb)) * p.nkv + head];
-    }
-#pragma unroll
-    for (int u = 0; u < KR_UNROLL; u++) {
-        if (!on[u]) continue;
-        const float f = kv8_scale(s[u]);
-        uint32_t h[4];
-        kv8_decode4<I8>(c[u].x, h[0], h[1]);
-        kv8_decode4<I8>(c[u].y, h[2], h[3]);
-        float2 y[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            y[i] = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
-            y[i].x *= f; y[i].y *= f;
+        for (int u = 0; u < KR_ROWS; u++) {
+            const int64_t j = j0 + u * step, row = pos + j;
+            if (j >= end || row < 0) continue;
+            c[u] = *reinterpret_cast<const uint2 *>(codes + (row * pieces + at) * PER);
+            s[u] = scales[(row >> p.lb) * p.nkv + head];
         }
-        const int64_t id = first + u * KR_THREADS;
-        if constexpr (F32) {
-            float4 *o = reinterpret_cast<float4 *>(out + id * PER * 4);
-            o[0] = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
-            o[1] = make_float4(y[2].x, y[2].y, y[3].x, y[3].y);
-        } else {
-            uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = pack_bf16x2(y[i].x, y[i].y);       // exact
-            *reinterpret_cast<uint4 *>(out + id * PER * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int u = 0; u < KR_ROWS; u++) {
+            const int64_t j = j0 + u * step;
+            if (j >= end || pos + j < 0) continue;
+            const float f = kv8_scale(s[u]);
+            uint32_t h[4];
+            kv8_decode4<I8>(c[u].x, h[0], h[1]);
+            kv8_decode4<I8>(c[u].y, h[2], h[3]);
+            float2 y[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                y[i] = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
+                y[i].x *= f; y[i].y *= f;
+            }
+            if constexpr (F32) {
+                float4 *o = reinterpret_cast<float4 *>(out + (j * pieces + at) * PER * 4);
+                o[0] = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
+                o[1] = make_float4(y[2].x, y[2].y, y[3].x, y[3].y);
+            } else {
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = pack_bf16x2(y[i].x, y[i].y);       // exact
+                *reinterpret_cast<uint4 *>(out + (j * pieces + at) * PER * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
         }
     }
 }
@@ -341,36 +391,40 @@ __global__ void __launch_bounds__(KR_THREADS) kv8_read_kernel(const Kv8ReadParam
 int log2_of(int block) { return block == 32 ? 5 : block == 64 ? 6 : 7; }
 
 int launch_read(cwk_ctx *ctx, const Kv8ReadParams &p, int hd, bool i8, bool f32) {
-    const int64_t pieces = (int64_t)p.B * p.n * p.nkv * (hd / 8);
-    const int64_t blocks = (pieces + KR_THREADS * KR_UNROLL - 1) / (KR_THREADS * KR_UNROLL);
-    if (blocks > 0x7FFFFFFF) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "kv8_load: too many rows in one call");
+    const int per_block = std::max(KR_THREADS / (p.nkv * (hd / 8)), 1) * KR_ROWS;
+    const int64_t chunks = (p.n + per_block - 1) / per_block;
+    if (chunks > 0x7FFFFFFF || p.B > 65535) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "kv8_load: too many rows or slots in one call");
     void (*kern)(Kv8ReadParams);
     if (hd == 256) kern = i8 ? (f32 ? kv8_read_kernel<256, true, true> : kv8_read_kernel<256, true, false>)
                              : (f32 ? kv8_read_kernel<256, false, true> : kv8_read_kernel<256, false, false>);
     else kern = i8 ? (f32 ? kv8_read_kernel<128, true, true> : kv8_read_kernel<128, true, false>)
                    : (f32 ? kv8_read_kernel<128, false, true> : kv8_read_kernel<128, false, false>);
-    CWK_CUDA(ctx, cwk_launch_early(kern, dim3((unsigned)blocks, 2), dim3(KR_THREADS), 0, ctx->stream, p));
+    CWK_CUDA(ctx, cwk_launch_early(kern, dim3((unsigned)chunks, p.B, 2), dim3(KR_THREADS), 0, ctx->stream, p));
     ctx->launches++;
     return CWK_OK;
 }
 
-template <int V, int SRC, bool PREP>
-int launch_write(cwk_ctx *ctx, Kv8WriteParams &p, int type) {
-    const int block = 1 << p.lb, warps = (std::min(block, p.n) + KW_ROWS - 1) / KW_ROWS;
+template <int V, int SRC, bool PREP, int ROWS>
+int launch_write_rows(cwk_ctx *ctx, Kv8WriteParams &p, int type) {
+    const int block = 1 << p.lb, warps = (std::min(block, p.n) + ROWS - 1) / ROWS;
     p.window = (int)(((int64_t)p.n + block - 2) / block + 1);
     p.tasks = (int64_t)2 * p.B * p.window * p.nkv;
     int64_t blocks = p.tasks;
     size_t smem = 0;
     if (PREP) {
-        p.heads = p.n * (int64_t)p.B * p.nh <= 16 * 1024 ? 1 : 4;      // query heads that share a token's angles; few rows: one warp each
+        p.heads = p.n * (int64_t)p.B * p.nh <= 16 * 1024 ? 1 : KQ_HEADS;      // query heads that share a token's angles; few rows: one warp each
         blocks += ((int64_t)p.B * p.n * ((p.nh + p.heads - 1) / p.heads) + warps - 1) / warps;
-        smem = (size_t)warps * (p.rot / 2) * sizeof(double2);
+        smem = (size_t)(warps + 1) * (p.rot / 2) * sizeof(double2) + (p.rot / 2) * sizeof(double);
     }
     if (blocks > 0x7FFFFFFF) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "kv8 write: too many rows in one call");
-    auto kern = type == CWK_KV8_INT8 ? kv8_write_kernel<V, SRC, true, PREP> : kv8_write_kernel<V, SRC, false, PREP>;
+    auto kern = type == CWK_KV8_INT8 ? kv8_write_kernel<V, SRC, true, PREP, ROWS> : kv8_write_kernel<V, SRC, false, PREP, ROWS>;
     CWK_CUDA(ctx, cwk_launch_early(kern, dim3((unsigned)blocks), dim3(32 * warps), smem, ctx->stream, p));
     ctx->launches++;
     return CWK_OK;
+}
+template <int V, int SRC, bool PREP>
+int launch_write(cwk_ctx *ctx, Kv8WriteParams &p, int type) {
+    return p.lb == 7 ? launch_write_rows<V, SRC, PREP, 8>(ctx, p, type) : launch_write_rows<V, SRC, PREP, 4>(ctx, p, type);
 }
 
 void describe(Kv8WriteParams &p, const cwk_kv8 *c, const void *k, const void *v, const int32_t *pos, const int32_t *count, int B, int n) {
@@ -445,7 +499,10 @@ int cwk_gqa_qk_prep_kv8(cwk_ctx *ctx, const float *qg, const float *k, const flo
     Kv8WriteParams p{};
     describe(p, c, k, v, pos, count, B, n);
     p.qg = qg; p.q_norm = q_norm; p.k_norm = k_norm; p.q_out = (uint16_t *)q_out; p.nh = nh; p.rot = rot; p.eps = eps;
-    for (int i = 0; i < rot / 2; i++) p.inv_freq[i] = pow(theta, -2.0 * i / rot);
+    for (int i = 0; i < rot / 2; i++) {
+        p.freq[i] = pow(theta, -2.0 * i / rot);
+        p.turn[i] = make_double2(cos(p.freq[i]), sin(p.freq[i]));
+    }
     CwkKernelTimer timer(ctx);
     return c->hd == 256 ? launch_write<8, SRC_F32, true>(ctx, p, c->type) : launch_write<4, SRC_F32, true>(ctx, p, c->type);
 }
