@@ -27,8 +27,7 @@ struct Kv8WriteParams {
     float eps;
     int64_t tasks;                             // K and V tasks; the blocks behind them have query rows
     int heads;                                 // query heads per warp
-    double freq[128];                          // angle of a pair per position
-    double2 turn[128];                         // its cos and sin
+    double freq_hi[16], freq_lo[8];            // angle per position of pair i: freq_hi[i / 8] * freq_lo[i % 8]
 };
 constexpr int KQ_HEADS = 4;                    // most query heads of a warp
 
@@ -72,53 +71,97 @@ __device__ __forceinline__ uint32_t finite_magnitude(float x) {
     return u < 0x7F800000u ? u : 0u;
 }
 
-// cos and sin of a position's angles, for the rot / 2 pairs of a head, by a warp into its share of shared memory
-__device__ __forceinline__ void angles(const double *freq, int pairs, int64_t pos, int lane, double2 *cs) {
-    for (int i = lane; i < pairs; i += 32) {
-        double c, s;
-        sincos((double)pos * freq[i], &s, &c);
-        cs[i] = make_double2(c, s);
+// float -> double in integer work: the conversion instructions of 64-bit types run at a small part of the rate of the arithmetic (with
+// them the keys of 2100 tokens took 38 us, most of the time in conversions). Subnormals are zero.
+__device__ __forceinline__ double wide(float x) {
+    const uint32_t u = __float_as_uint(x), e = u & 0x7F800000u, sign = u & 0x80000000u;
+    const uint32_t hi = sign | (((u & 0x7FFFFFFFu) >> 3) + 0x38000000u) | (e == 0x7F800000u ? 0x7FF00000u : 0u);
+    return __hiloint2double((int)(e ? hi : sign), (int)(e ? u << 29 : 0u));
+}
+template <class T> __device__ __forceinline__ T as(float x);
+template <> __device__ __forceinline__ float as<float>(float x) { return x; }
+template <> __device__ __forceinline__ double as<double>(float x) { return wide(x); }
+
+// Angles per position of this lane's pairs lane, lane + 32, ..
+struct Freq {
+    double f[4];
+    __device__ __forceinline__ Freq(const Kv8WriteParams &p, int pairs, int lane) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = lane + 32 * k;
+            f[k] = i < pairs ? p.freq_hi[i >> 3] * p.freq_lo[i & 7] : 0.0;
+        }
+    }
+};
+// cos and sin of a position's angles by a warp, for all its lanes. In float: the angle taken into [-pi, pi] in double, then rounded
+// (2^-22); the sum with 1.5 * 2^52 is the nearest whole number of turns.
+__device__ __forceinline__ void angles(const Freq &q, int pairs, int64_t pos, int lane, float2 *cs) {
+    const double at = (double)pos;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if (32 * k >= pairs) break;
+        const double a = at * q.f[k], turns = (a * 0.15915494309189533577 + 6755399441055744.0) - 6755399441055744.0;
+        float s, c;
+        sincosf((float)fma(-turns, 6.283185307179586477, a), &s, &c);
+        if (lane + 32 * k < pairs) cs[lane + 32 * k] = make_float2(c, s);
     }
     __syncwarp();
 }
-// ... and of the next position: a turn by the angle of one. (At most seven in a row: an error of some 2^-50.)
-__device__ __forceinline__ void next_angles(const double2 *turn, int pairs, int lane, double2 *cs) {
+__device__ __forceinline__ void angles(const Freq &q, int pairs, int64_t pos, int lane, double2 *cs) {
     __syncwarp();
-    for (int i = lane; i < pairs; i += 32) {
-        const double2 a = cs[i], b = turn[i];
-        cs[i] = make_double2(a.x * b.x - a.y * b.y, a.y * b.x + a.x * b.y);
+#pragma unroll 1
+    for (int k = 0; 32 * k < pairs; k++) {
+        double c, s;
+        sincos((double)pos * (k == 0 ? q.f[0] : k == 1 ? q.f[1] : k == 2 ? q.f[2] : q.f[3]), &s, &c);
+        if (lane + 32 * k < pairs) cs[lane + 32 * k] = make_double2(c, s);
     }
     __syncwarp();
 }
 
-// A row's norm and rotation by a warp: y = x * rstd * (1 + w), the first `rot` values turned in pairs (i, i + rot / 2). Keys in T = double:
-// a code hangs on which side of a border a value is, and this way it is the definition's; queries, which are rounded to bf16, in float.
-template <int V, class T, class X>
-__device__ __forceinline__ void norm_rotate(const X &x, T rstd, const T (&w1)[V], int rot, int lane, const double2 *cs, T (&y)[V]) {
-#pragma unroll
-    for (int i = 0; i < V; i++) y[i] = (T)x[i] * rstd * w1[i];
-    if (rot == 0) return;
+// A row's norm and rotation by a warp: y = x * rstd * (1 + w), the first `rot` values turned in pairs (i, i + rot / 2). In float every value is
+// within KEY_ERR times the size of its pair: sum of squares 8 roundings (half of that in its root), root and quotient 2, 1 + w, two
+// products, angle 4 + 2, cos and sin 1, turn 3, in all 19 of 2^-24, < 2^-19; of the result's size |y| + |other|, which is at least 1 / sqrt 2 of
+// the pair's, < 2^-18.
+constexpr float KEY_ERR = 0x1p-18f;
+// the lane with the other values of this lane's pairs (itself where it has none)
+template <int V>
+__device__ __forceinline__ int partner(int rot, int lane) {
     const int d0 = lane * V, shift = rot / 2 / V;
+    return d0 < rot / 2 ? lane + shift : d0 < rot ? lane - shift : lane;
+}
+template <int V, class T, class X, class CS>
+__device__ __forceinline__ void norm_rotate(const X &x, T rstd, const T (&w1)[V], int rot, int lane, const CS *cs, T (&y)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) y[i] = as<T>(x[i]) * rstd * w1[i];
+    if (rot == 0) return;
+    const int d0 = lane * V, from = partner<V>(rot, lane), pair = d0 < rot / 2 ? d0 : d0 - rot / 2;
     const bool lo = d0 < rot / 2, hi = !lo && d0 < rot;
-    const int from = lo ? lane + shift : hi ? lane - shift : lane, pair = lo ? d0 : hi ? d0 - rot / 2 : 0;
 #pragma unroll
     for (int i = 0; i < V; i++) {
         const T other = __shfl_sync(0xffffffffu, y[i], from);
         if (lo || hi) {
-            const double2 t = cs[pair + i];
-            const T c = (T)t.x, s = lo ? -(T)t.y : (T)t.y;
-            y[i] = y[i] * c + other * s;
+            const CS t = cs[pair + i];
+            y[i] = y[i] * t.x + other * (lo ? -t.y : t.y);
         }
     }
 }
+// this lane's part of a row's sum of squares, and the sum over the warp
 template <int V, class T, class X>
-__device__ __forceinline__ T row_rstd(const X &x, float eps) {
+__device__ __forceinline__ T squares(const X &x) {
     T sum = 0;
 #pragma unroll
-    for (int i = 0; i < V; i++) sum += (T)x[i] * (T)x[i];
+    for (int i = 0; i < V; i += 4) {
+        const T a = as<T>(x[i]), b = as<T>(x[i + 1]), c = as<T>(x[i + 2]), d = as<T>(x[i + 3]);
+        sum += (a * a + b * b) + (c * c + d * d);
+    }
+    return sum;
+}
+template <class T>
+__device__ __forceinline__ T warp_sum(T sum) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return (T)1 / sqrt(sum / (T)(32 * V) + (T)eps);
+    return sum;
 }
 
 // double -> float for a second rounding to few bits: cut off, the last bit set where anything was, so that the second rounding sees
@@ -136,8 +179,7 @@ __device__ __forceinline__ void store_words(uint8_t *dst, const uint32_t (&w)[V 
 }
 // Codes of values in units of the scale. careful: some are not finite, or larger than the largest code.
 template <int V, bool I8>
-__device__ __forceinline__ void store_codes(uint8_t *dst, const float (&y)[V], bool careful, bool is_v) {
-    uint32_t w[V / 4];
+__device__ __forceinline__ void codes_of(const float (&y)[V], bool careful, bool is_v, uint32_t (&w)[V / 4]) {
 #pragma unroll
     for (int i = 0; i < V / 4; i++) {
         float t[4] = {y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
@@ -154,66 +196,84 @@ __device__ __forceinline__ void store_codes(uint8_t *dst, const float (&y)[V], b
             w[i] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
         } else w[i] = kv8_encode4<I8>(t);
     }
+}
+template <int V, bool I8>
+__device__ __forceinline__ void store_codes(uint8_t *dst, const float (&y)[V], bool careful, bool is_v) {
+    uint32_t w[V / 4];
+    codes_of<V, I8>(y, careful, is_v, w);
     store_words<V>(dst, w);
 }
 
-// Rows r0 .. r0 + lead - 1 of an open block move from scale 2^was to 2^e, e > was.
-template <int V, bool I8>
-__device__ __forceinline__ void rescale(uint8_t *codes, int64_t ld, int lead, int was, int e, bool is_v, int warp, int warps, int lane) {
+// Rows r0 .. r0 + lead - 1 of an open block move from scale 2^was to 2^e, e > was: 16 codes a thread, two such pieces in flight (one warp
+// may have 127 rows to move).
+template <int HD, bool I8>
+__device__ __forceinline__ void rescale(uint8_t *codes, int64_t ld, int lead, int was, int e, bool is_v) {
+    constexpr int CH = HD / 16, U = 2;
     const float f = was - e < -126 ? 0.f : kv8_two(was - e);
-    for (int r = warp; r < lead; r += warps) {
-        uint8_t *at = codes + r * ld + lane * V;
-        float y[V];
+    for (int i0 = threadIdx.x; i0 < lead * CH; i0 += U * blockDim.x) {
+        uint4 c[U];
 #pragma unroll
-        for (int i = 0; i < V / 4; i++) {
-            uint32_t a, b;
-            kv8_decode4<I8>(*reinterpret_cast<const uint32_t *>(at + 4 * i), a, b);
-            const float2 u = __half22float2(*reinterpret_cast<const __half2 *>(&a)), v = __half22float2(*reinterpret_cast<const __half2 *>(&b));
-            y[4 * i] = u.x * f; y[4 * i + 1] = u.y * f; y[4 * i + 2] = v.x * f; y[4 * i + 3] = v.y * f;
+        for (int u = 0; u < U; u++) {
+            const int i = i0 + u * blockDim.x;
+            if (i < lead * CH) c[u] = *reinterpret_cast<const uint4 *>(codes + (i / CH) * ld + (i % CH) * 16);
         }
-        store_codes<V, I8>(at, y, true, is_v);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = i0 + u * blockDim.x;
+            if (i >= lead * CH) break;
+            uint8_t *at = codes + (i / CH) * ld + (i % CH) * 16;
+            const uint32_t w[4] = {c[u].x, c[u].y, c[u].z, c[u].w};
+#pragma unroll
+            for (int k = 0; k < 4; k += 2) {
+                float y[8];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t a, b;
+                    kv8_decode4<I8>(w[k + h], a, b);
+                    const float2 v0 = __half22float2(*reinterpret_cast<const __half2 *>(&a)), v1 = __half22float2(*reinterpret_cast<const __half2 *>(&b));
+                    y[4 * h] = v0.x * f; y[4 * h + 1] = v0.y * f; y[4 * h + 2] = v1.x * f; y[4 * h + 3] = v1.y * f;
+                }
+                store_codes<8, I8>(at + 4 * k, y, true, is_v);
+            }
+        }
     }
 }
 
 // V: values of a row per lane (head dim / 32); ROWS: rows of a warp. PREP: f32 rows, keys normed and rotated; blocks from p.tasks on have
 // query rows.
 template <int V, int SRC, bool I8, bool PREP, int ROWS>
-__global__ void __launch_bounds__(512) kv8_write_kernel(const __grid_constant__ Kv8WriteParams p) {
+__global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel(const __grid_constant__ Kv8WriteParams p) {
     constexpr int HD = 32 * V;
-    extern __shared__ double2 s_dyn[];                     // PREP: [warp][rot / 2] cos and sin, [rot / 2] turns, [rot / 2] frequencies
+    extern __shared__ double2 s_cs[];                      // PREP: [warp][rot / 2] cos and sin of a position
     __shared__ uint32_t s_max[16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int pairs = p.rot / 2;
-    double2 *cs = s_dyn + warp * pairs, *turn = s_dyn + warps * pairs;
-    double *freq = reinterpret_cast<double *>(turn + pairs);
+    double2 *cs = s_cs + warp * pairs;
+    float2 *csf = reinterpret_cast<float2 *>(cs);          // (one of them at a time)
     cwk_pdl_launch();
-    if (PREP) {
-        for (int i = threadIdx.x; i < pairs; i += blockDim.x) { turn[i] = p.turn[i]; freq[i] = p.freq[i]; }
-        __syncthreads();
-    }
     cwk_pdl_wait();
     if (PREP && blockIdx.x >= p.tasks) {
         // ---- query rows: a warp has `heads` heads of one token
         const int parts = (p.nh + p.heads - 1) / p.heads;
         const int64_t id = ((int64_t)blockIdx.x - p.tasks) * warps + warp, t = id / parts;
         if (t >= (int64_t)p.B * p.n) return;
-        const int b = (int)(t / p.n), j = (int)(t % p.n), h0 = (int)(id % parts) * p.heads, mine = min(p.heads, p.nh - h0);
+        const int b = (int)(t / p.n), j = (int)(t % p.n), h0 = (int)(id % parts) * p.heads, heads = min(p.heads, p.nh - h0);
         Raw<V, SRC_F32> x[KQ_HEADS], w;
         w.load(p.q_norm, 0, lane);
 #pragma unroll
         for (int i = 0; i < KQ_HEADS; i++)
-            if (i < mine) x[i].load(p.qg, (t * p.nh + h0 + i) * 2, lane);      // rows [q | gate] of 2 * hd
+            if (i < heads) x[i].load(p.qg, (t * p.nh + h0 + i) * 2, lane);      // rows [q | gate] of 2 * hd
         int64_t pos;
         if (j >= new_rows(p, b, pos)) return;
-        angles(freq, pairs, pos + j, lane, cs);
+        angles(Freq(p, pairs, lane), pairs, pos + j, lane, csf);
         float w1[V];
 #pragma unroll
         for (int i = 0; i < V; i++) w1[i] = 1.f + w[i];
 #pragma unroll
         for (int i = 0; i < KQ_HEADS; i++) {
-            if (i >= mine) break;
+            if (i >= heads) break;
             float y[V];
-            norm_rotate<V, float>(x[i], row_rstd<V, float>(x[i], p.eps), w1, p.rot, lane, cs, y);
+            norm_rotate<V, float>(x[i], 1.f / sqrtf(warp_sum(squares<V, float>(x[i])) / (float)HD + p.eps), w1, p.rot, lane, csf, y);
             uint32_t o[V / 2];
 #pragma unroll
             for (int k = 0; k < V / 2; k++) o[k] = pack_bf16x2(y[2 * k], y[2 * k + 1]);
@@ -233,93 +293,156 @@ __global__ void __launch_bounds__(512) kv8_write_kernel(const __grid_constant__ 
     const int64_t blk = (pos >> p.lb) + win, r0 = blk << p.lb;
     const int64_t lo = max(r0, pos), hi = min(r0 + (1 << p.lb), pos + cnt);
     if (lo >= hi) return;
-    const bool norm = PREP && !is_v;
     uint8_t *codes = (is_v ? p.vc : p.kc) + (((int64_t)b * p.rows + r0) * p.nkv + head) * HD;
     uint8_t *scale = (is_v ? p.vs : p.ks) + ((int64_t)b * (p.rows >> p.lb) + blk) * p.nkv + head;
     const int64_t ld = (int64_t)p.nkv * HD;
     const int lead = (int)(lo - r0), many = (int)(hi - lo);
     const int was_byte = lead > 0 ? (int)*scale : 0;
-    const int first = warp * ROWS;                         // this warp's rows: lo + first .. + ROWS - 1, those below hi
+    const int first = warp * ROWS, mine = min(ROWS, many - first);      // this warp's rows: lo + first .. (none: <= 0)
+    const void *src = is_v ? p.v : p.k;
+    const int64_t row = ((int64_t)b * p.n + (lo - pos) + first) * p.nkv + head;
+    // over the task: the largest of a value's bits
+    auto task_max = [&](uint32_t m) {
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (lane == 0) s_max[warp] = m;
+        __syncthreads();
+        for (int i = 0; i < warps; i++) m = max(m, s_max[i]);
+        return m;
+    };
+    int e;
+    bool careful;                                          // some values are not finite, or larger than the largest code
+    auto settle = [&](uint32_t amax, bool odd) {
+        e = kv8_exponent(__uint_as_float(amax), I8);
+        careful = odd || e == kv8_high(I8);
+        if (lead > 0) {
+            const int was = min(max(was_byte - 127, KV8_LOW), kv8_high(I8));
+            if (was >= e) e = was;
+            else rescale<HD, I8>(codes, ld, lead, was, e, is_v);
+        }
+        if (threadIdx.x == 0) *scale = (uint8_t)(e + 127);
+    };
+    uint8_t *dst = codes + (lead + first) * ld + lane * V;
     Raw<V, SRC> x[ROWS];
-    double w1[V], rstd[ROWS];
-    uint32_t amax = 0;
-    {
-        const void *src = is_v ? p.v : p.k;
-        const int64_t row = ((int64_t)b * p.n + (lo - pos) + first) * p.nkv + head;
 #pragma unroll
-        for (int i = 0; i < ROWS; i++)
-            if (first + i < many) x[i].load(src, row + i * p.nkv, lane);
-    }
-    if (norm) {
+    for (int i = 0; i < ROWS; i++)
+        if (i < mine) x[i].load(src, row + i * p.nkv, lane);
+    if (PREP && !is_v) {
+        // ---- keys. A code is that of the value in 64 bits, formed in float: where a float's error could change the code (or the
+        // exponent), the row (or the largest magnitude) is formed again in double. That is one row in ten or less, and double, with its
+        // conversions, is some eight times the work: 512 tokens 20 us with all rows in double.
+        const Freq freq(p, pairs, lane);
         Raw<V, SRC_F32> w;
         w.load(p.k_norm, 0, lane);
+        auto row64 = [&](int r, double (&y)[V]) {
+            Raw<V, SRC> z;
+            z.load(src, row + r * p.nkv, lane);
+            double w1[V];
 #pragma unroll
-        for (int i = 0; i < V; i++) w1[i] = 1.0 + (double)w[i];
-        if (first < many) angles(freq, pairs, lo + first, lane, cs);
-    }
-    uint32_t all = 0;                                      // as amax, of all values
+            for (int i = 0; i < V; i++) w1[i] = 1.0 + wide(w[i]);
+            angles(freq, pairs, lo + first + r, lane, cs);
+            norm_rotate<V, double>(z, rsqrt(warp_sum(squares<V, double>(z)) / (double)HD + (double)p.eps), w1, p.rot, lane, cs, y);
+        };
+        float y[ROWS][V];
+        uint32_t amax = 0;
+        bool unsure = false;
+        {
+            float w1[V];
 #pragma unroll
-    for (int i = 0; i < ROWS; i++) {
-        if (first + i >= many) continue;                   // (the same for the whole warp)
-        if (norm) {
-            double y[V];
-            rstd[i] = row_rstd<V, double>(x[i], p.eps);
-            if (i > 0) next_angles(turn, pairs, lane, cs);
-            norm_rotate<V, double>(x[i], rstd[i], w1, p.rot, lane, cs, y);
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float up = __double2float_ru(fabs(y[j]));      // never below the value
-                amax = max(amax, finite_magnitude(up));
-                all = max(all, __float_as_uint(up) & 0x7FFFFFFFu);
-            }
-        } else all = max(all, x[i].magnitude());
-    }
-    if (!norm) {
-        amax = all;
-        if (all >= 0x7F800000u) {                          // an infinity saturates and does not set the scale; nor does a NaN
-            amax = 0;
+            for (int i = 0; i < V; i++) w1[i] = 1.f + w[i];
 #pragma unroll
             for (int i = 0; i < ROWS; i++) {
-                if (first + i >= many) continue;
+                if (i >= mine) break;
+                const float r = 1.f / sqrtf(warp_sum(squares<V, float>(x[i])) / (float)HD + p.eps);
+                unsure |= !(r > 1e-15f && r < 1e30f);      // (where squares leave the range or are too small for it)
+                angles(freq, pairs, lo + first + i, lane, csf);
+                norm_rotate<V, float>(x[i], r, w1, p.rot, lane, csf, y[i]);
 #pragma unroll
-                for (int j = 0; j < V; j++) amax = max(amax, finite_magnitude(x[i][j]));
+                for (int j = 0; j < V; j++) amax = max(amax, __float_as_uint(y[i][j]) & 0x7FFFFFFFu);
             }
         }
-    }
-    amax = __reduce_max_sync(0xffffffffu, amax);
-    if (lane == 0) s_max[warp] = amax;
-    const bool odd = __syncthreads_or(all >= 0x7F800000u);
-    for (int i = 0; i < warps; i++) amax = max(amax, s_max[i]);
-    int e = kv8_exponent(__uint_as_float(amax), I8);
-    const bool careful = odd || e == kv8_high(I8);
-    if (lead > 0) {
-        const int was = min(max(was_byte - 127, KV8_LOW), kv8_high(I8));
-        if (was >= e) e = was;
-        else rescale<V, I8>(codes, ld, lead, was, e, is_v, warp, warps, lane);
-    }
-    if (threadIdx.x == 0) *scale = (uint8_t)(e + 127);
-    const float f = kv8_two(-e);
-    uint8_t *dst = codes + (lead + first) * ld + lane * V;
-    if (norm && first < many) angles(freq, pairs, lo + first, lane, cs);
+        amax = task_max(amax);
+        const float top = __uint_as_float(amax);
+        bool odd = false;
+        unsure |= amax >= 0x7F800000u;
+        const bool all64 = __syncthreads_or(unsure);       // no row's float values are good
+        if (all64 || kv8_exponent(top * (1.f - 2.f * KEY_ERR), I8) != kv8_exponent(top * (1.f + 2.f * KEY_ERR), I8)) {
+            uint32_t finite = 0, all = 0;
+#pragma unroll 1
+            for (int r = 0; r < mine; r++) {
+                double z[V];
+                row64(r, z);
 #pragma unroll
-    for (int i = 0; i < ROWS; i++, dst += ld) {
-        if (first + i >= many) continue;
-        float y[V];
-        if (norm) {
-            double z[V];
-            if (i > 0) next_angles(turn, pairs, lane, cs);
-            norm_rotate<V, double>(x[i], rstd[i], w1, p.rot, lane, cs, z);
-            // INT8: the nearest whole number, as a float; E4M3: to odd, then (in store_codes) to nearest
+                for (int j = 0; j < V; j++) {
+                    const float up = __double2float_ru(fabs(z[j]));      // never below the value
+                    finite = max(finite, finite_magnitude(up));
+                    all = max(all, __float_as_uint(up) & 0x7FFFFFFFu);
+                }
+            }
+            odd = __syncthreads_or(all >= 0x7F800000u);
+            amax = task_max(finite);
+        }
+        settle(amax, odd);
+        const float f = kv8_two(-e);
+        uint32_t again = 0;                                // rows of which some value's code is not certain
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+            if (i >= mine) break;
+            float a[V], b[V];
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                if constexpr (I8) y[j] = careful ? (z[j] == z[j] ? (float)rint(fmin(fmax(z[j] * (double)f, -127.0), 127.0)) : 0.f)
-                                                 : (float)__double2loint(z[j] * (double)f + 6755399441055744.0);      // (plus 1.5 * 2^52)
-                else y[j] = to_odd(z[j] * (double)f);
+                const float other = __shfl_sync(0xffffffffu, y[i][j], partner<V>(p.rot, lane));
+                const float err = (fabsf(y[i][j]) + fabsf(other)) * KEY_ERR;
+                a[j] = (y[i][j] - err) * f;
+                b[j] = (y[i][j] + err) * f;
             }
-        } else {
+            // what lies between two values of one code has that code
+            uint32_t wa[V / 4], wb[V / 4], differ = 0;
+            codes_of<V, I8>(a, careful, false, wa);
+            codes_of<V, I8>(b, careful, false, wb);
 #pragma unroll
-            for (int j = 0; j < V; j++) y[j] = x[i][j] * f;
+            for (int j = 0; j < V / 4; j++) differ |= wa[j] ^ wb[j];
+            if (all64 || __any_sync(0xffffffffu, differ != 0)) again |= 1u << i;
+            else store_words<V>(dst + i * ld, wa);
         }
+        const double f64 = wide(f);
+#pragma unroll 1
+        for (; again; again &= again - 1) {
+            const int r = __ffs(again) - 1;
+            double z[V];
+            row64(r, z);
+            float q[V];
+            // INT8: the nearest whole number, as a float; E4M3: to odd, then (in codes_of) to nearest
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                if constexpr (I8) q[j] = z[j] == z[j] ? (float)rint(fmin(fmax(z[j] * f64, -127.0), 127.0)) : 0.f;
+                else q[j] = to_odd(z[j] * f64);
+            }
+            store_codes<V, I8>(dst + r * ld, q, true, false);
+        }
+        return;
+    }
+    uint32_t all = 0;
+#pragma unroll
+    for (int i = 0; i < ROWS; i++)
+        if (i < mine) all = max(all, x[i].magnitude());
+    uint32_t amax = all;
+    if (all >= 0x7F800000u) {                              // an infinity saturates and does not set the scale; nor does a NaN
+        amax = 0;
+#pragma unroll
+        for (int i = 0; i < ROWS; i++)
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (i < mine) amax = max(amax, finite_magnitude(x[i][j]));
+    }
+    const bool odd = __syncthreads_or(all >= 0x7F800000u);
+    settle(task_max(amax), odd);
+    const float f = kv8_two(-e);
+#pragma unroll
+    for (int i = 0; i < ROWS; i++, dst += ld) {
+        if (i >= mine) break;
+        float y[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) y[j] = x[i][j] * f;
         store_codes<V, I8>(dst, y, careful, is_v);
     }
 }
@@ -411,20 +534,21 @@ int launch_write_rows(cwk_ctx *ctx, Kv8WriteParams &p, int type) {
     p.tasks = (int64_t)2 * p.B * p.window * p.nkv;
     int64_t blocks = p.tasks;
     size_t smem = 0;
+    auto kern = type == CWK_KV8_INT8 ? kv8_write_kernel<V, SRC, true, PREP, ROWS> : kv8_write_kernel<V, SRC, false, PREP, ROWS>;
     if (PREP) {
         p.heads = p.n * (int64_t)p.B * p.nh <= 16 * 1024 ? 1 : KQ_HEADS;      // query heads that share a token's angles; few rows: one warp each
         blocks += ((int64_t)p.B * p.n * ((p.nh + p.heads - 1) / p.heads) + warps - 1) / warps;
-        smem = (size_t)(warps + 1) * (p.rot / 2) * sizeof(double2) + (p.rot / 2) * sizeof(double);
+        smem = (size_t)(p.rot / 2) * warps * sizeof(double2);      // 32 KB at most
     }
     if (blocks > 0x7FFFFFFF) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "kv8 write: too many rows in one call");
-    auto kern = type == CWK_KV8_INT8 ? kv8_write_kernel<V, SRC, true, PREP, ROWS> : kv8_write_kernel<V, SRC, false, PREP, ROWS>;
     CWK_CUDA(ctx, cwk_launch_early(kern, dim3((unsigned)blocks), dim3(32 * warps), smem, ctx->stream, p));
     ctx->launches++;
     return CWK_OK;
 }
+// Rows of a warp: eight, and four for the preparation of shorter blocks, whose keys go from row to row.
 template <int V, int SRC, bool PREP>
 int launch_write(cwk_ctx *ctx, Kv8WriteParams &p, int type) {
-    return p.lb == 7 ? launch_write_rows<V, SRC, PREP, 8>(ctx, p, type) : launch_write_rows<V, SRC, PREP, 4>(ctx, p, type);
+    return p.lb == 7 || !PREP ? launch_write_rows<V, SRC, PREP, 8>(ctx, p, type) : launch_write_rows<V, SRC, PREP, 4>(ctx, p, type);
 }
 
 void describe(Kv8WriteParams &p, const cwk_kv8 *c, const void *k, const void *v, const int32_t *pos, const int32_t *count, int B, int n) {
@@ -499,9 +623,9 @@ int cwk_gqa_qk_prep_kv8(cwk_ctx *ctx, const float *qg, const float *k, const flo
     Kv8WriteParams p{};
     describe(p, c, k, v, pos, count, B, n);
     p.qg = qg; p.q_norm = q_norm; p.k_norm = k_norm; p.q_out = (uint16_t *)q_out; p.nh = nh; p.rot = rot; p.eps = eps;
-    for (int i = 0; i < rot / 2; i++) {
-        p.freq[i] = pow(theta, -2.0 * i / rot);
-        p.turn[i] = make_double2(cos(p.freq[i]), sin(p.freq[i]));
+    if (rot > 0) {
+        for (int i = 0; i < 16; i++) p.freq_hi[i] = pow(theta, -16.0 * i / rot);
+        for (int i = 0; i < 8; i++) p.freq_lo[i] = pow(theta, -2.0 * i / rot);
     }
     CwkKernelTimer timer(ctx);
     return c->hd == 256 ? launch_write<8, SRC_F32, true>(ctx, p, c->type) : launch_write<4, SRC_F32, true>(ctx, p, c->type);
