@@ -82,48 +82,42 @@ template <class T> __device__ __forceinline__ T as(float x);
 template <> __device__ __forceinline__ float as<float>(float x) { return x; }
 template <> __device__ __forceinline__ double as<double>(float x) { return wide(x); }
 
-// Angles per position of this lane's pairs lane, lane + 32, ..
-struct Freq {
-    double f[4];
-    __device__ __forceinline__ Freq(const Kv8WriteParams &p, int pairs, int lane) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int i = lane + 32 * k;
-            f[k] = i < pairs ? p.freq_hi[i >> 3] * p.freq_lo[i & 7] : 0.0;
+// The angle of pair i per position.
+__device__ __forceinline__ double frequency(const Kv8WriteParams &p, int i) { return p.freq_hi[i >> 3] * p.freq_lo[i & 7]; }
+// cos and sin of the angles at positions pos .. pos + rows - 1 by a warp, [rows][pairs]: the angle taken into [-pi, pi] in double, then
+// rounded to float (2^-22); the sum with 1.5 * 2^52 is the nearest whole number of turns. (Not unrolled: the copies of the code that
+// forms a cosine would not stay in the instruction cache.)
+__device__ __forceinline__ void angles(const Kv8WriteParams &p, int pairs, int64_t pos, int rows, int lane, float2 *cs) {
+#pragma unroll 1
+    for (int i = lane; i < pairs; i += 32) {
+        const double f = frequency(p, i);
+#pragma unroll 1
+        for (int r = 0; r < rows; r++) {
+            const double a = (double)(pos + r) * f, turns = (a * 0.15915494309189533577 + 6755399441055744.0) - 6755399441055744.0;
+            float s, c;
+            sincosf((float)fma(-turns, 6.283185307179586477, a), &s, &c);
+            cs[r * pairs + i] = make_float2(c, s);
         }
-    }
-};
-// cos and sin of a position's angles by a warp, for all its lanes. In float: the angle taken into [-pi, pi] in double, then rounded
-// (2^-22); the sum with 1.5 * 2^52 is the nearest whole number of turns.
-__device__ __forceinline__ void angles(const Freq &q, int pairs, int64_t pos, int lane, float2 *cs) {
-    const double at = (double)pos;
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        if (32 * k >= pairs) break;
-        const double a = at * q.f[k], turns = (a * 0.15915494309189533577 + 6755399441055744.0) - 6755399441055744.0;
-        float s, c;
-        sincosf((float)fma(-turns, 6.283185307179586477, a), &s, &c);
-        if (lane + 32 * k < pairs) cs[lane + 32 * k] = make_float2(c, s);
     }
     __syncwarp();
 }
-__device__ __forceinline__ void angles(const Freq &q, int pairs, int64_t pos, int lane, double2 *cs) {
+// the same of one position in double
+__device__ __forceinline__ void angles(const Kv8WriteParams &p, int pairs, int64_t pos, int lane, double2 *cs) {
     __syncwarp();
 #pragma unroll 1
-    for (int k = 0; 32 * k < pairs; k++) {
+    for (int i = lane; i < pairs; i += 32) {
         double c, s;
-        sincos((double)pos * (k == 0 ? q.f[0] : k == 1 ? q.f[1] : k == 2 ? q.f[2] : q.f[3]), &s, &c);
-        if (lane + 32 * k < pairs) cs[lane + 32 * k] = make_double2(c, s);
+        sincos((double)pos * frequency(p, i), &s, &c);
+        cs[i] = make_double2(c, s);
     }
     __syncwarp();
 }
 
-// A row's norm and rotation by a warp: y = x * rstd * (1 + w), the first `rot` values turned in pairs (i, i + rot / 2). In float every value is
-// within KEY_ERR times the size of its pair: sum of squares 8 roundings (half of that in its root), root and quotient 2, 1 + w, two
-// products, angle 4 + 2, cos and sin 1, turn 3, in all 19 of 2^-24, < 2^-19; of the result's size |y| + |other|, which is at least 1 / sqrt 2 of
-// the pair's, < 2^-18.
-constexpr float KEY_ERR = 0x1p-18f;
+// A row's norm and rotation by a warp: y = x * rstd * (1 + w), the first `rot` values turned in pairs (i, i + rot / 2). Errors of a value in
+// float, in units of 2^-24: sum of squares 8 roundings, in its root half of that, rsqrtf 4 (two units in the last place), its argument 1, 1 + w 1,
+// two products 2, in all 12 of the value's size: < 2^-20. A turned one: angle 4 (rounded from [-pi, pi]), cos and sin 2 (an ulp or two),
+// turn 3, in all 21 of the pair's size, which is at most sqrt 2 times the result's |y| + |other|: < 2^-19 of that.
+constexpr float KEY_ERR = 0x1p-20f, KEY_ERR_TURNED = 0x1p-19f;
 // the lane with the other values of this lane's pairs (itself where it has none)
 template <int V>
 __device__ __forceinline__ int partner(int rot, int lane) {
@@ -244,12 +238,12 @@ __device__ __forceinline__ void rescale(uint8_t *codes, int64_t ld, int lead, in
 template <int V, int SRC, bool I8, bool PREP, int ROWS>
 __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel(const __grid_constant__ Kv8WriteParams p) {
     constexpr int HD = 32 * V;
-    extern __shared__ double2 s_cs[];                      // PREP: [warp][rot / 2] cos and sin of a position
+    extern __shared__ double2 s_cs[];                      // PREP: of a warp, [ROWS][rot / 2] cos and sin in float, or [rot / 2] in double
     __shared__ uint32_t s_max[16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int pairs = p.rot / 2;
-    double2 *cs = s_cs + warp * pairs;
-    float2 *csf = reinterpret_cast<float2 *>(cs);          // (one of them at a time)
+    float2 *csf = reinterpret_cast<float2 *>(s_cs) + warp * ROWS * pairs;
+    double2 *cs = reinterpret_cast<double2 *>(csf);        // (one of them at a time)
     cwk_pdl_launch();
     cwk_pdl_wait();
     if (PREP && blockIdx.x >= p.tasks) {
@@ -265,7 +259,7 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
             if (i < heads) x[i].load(p.qg, (t * p.nh + h0 + i) * 2, lane);      // rows [q | gate] of 2 * hd
         int64_t pos;
         if (j >= new_rows(p, b, pos)) return;
-        angles(Freq(p, pairs, lane), pairs, pos + j, lane, csf);
+        angles(p, pairs, pos + j, 1, lane, csf);
         float w1[V];
 #pragma unroll
         for (int i = 0; i < V; i++) w1[i] = 1.f + w[i];
@@ -273,7 +267,7 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
         for (int i = 0; i < KQ_HEADS; i++) {
             if (i >= heads) break;
             float y[V];
-            norm_rotate<V, float>(x[i], 1.f / sqrtf(warp_sum(squares<V, float>(x[i])) / (float)HD + p.eps), w1, p.rot, lane, csf, y);
+            norm_rotate<V, float>(x[i], rsqrtf(warp_sum(squares<V, float>(x[i])) * (1.f / HD) + p.eps), w1, p.rot, lane, csf, y);
             uint32_t o[V / 2];
 #pragma unroll
             for (int k = 0; k < V / 2; k++) o[k] = pack_bf16x2(y[2 * k], y[2 * k + 1]);
@@ -328,9 +322,8 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
         if (i < mine) x[i].load(src, row + i * p.nkv, lane);
     if (PREP && !is_v) {
         // ---- keys. A code is that of the value in 64 bits, formed in float: where a float's error could change the code (or the
-        // exponent), the row (or the largest magnitude) is formed again in double. That is one row in ten or less, and double, with its
+        // exponent), the row (or the largest magnitude) is formed again in double. That is one row in thirty or less, and double, with its
         // conversions, is some eight times the work: 512 tokens 20 us with all rows in double.
-        const Freq freq(p, pairs, lane);
         Raw<V, SRC_F32> w;
         w.load(p.k_norm, 0, lane);
         auto row64 = [&](int r, double (&y)[V]) {
@@ -339,12 +332,13 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
             double w1[V];
 #pragma unroll
             for (int i = 0; i < V; i++) w1[i] = 1.0 + wide(w[i]);
-            angles(freq, pairs, lo + first + r, lane, cs);
+            angles(p, pairs, lo + first + r, lane, cs);
             norm_rotate<V, double>(z, rsqrt(warp_sum(squares<V, double>(z)) / (double)HD + (double)p.eps), w1, p.rot, lane, cs, y);
         };
         float y[ROWS][V];
         uint32_t amax = 0;
         bool unsure = false;
+        angles(p, pairs, lo + first, max(mine, 0), lane, csf);
         {
             float w1[V];
 #pragma unroll
@@ -352,10 +346,9 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
 #pragma unroll
             for (int i = 0; i < ROWS; i++) {
                 if (i >= mine) break;
-                const float r = 1.f / sqrtf(warp_sum(squares<V, float>(x[i])) / (float)HD + p.eps);
+                const float r = rsqrtf(warp_sum(squares<V, float>(x[i])) * (1.f / HD) + p.eps);
                 unsure |= !(r > 1e-15f && r < 1e30f);      // (where squares leave the range or are too small for it)
-                angles(freq, pairs, lo + first + i, lane, csf);
-                norm_rotate<V, float>(x[i], r, w1, p.rot, lane, csf, y[i]);
+                norm_rotate<V, float>(x[i], r, w1, p.rot, lane, csf + i * pairs, y[i]);
 #pragma unroll
                 for (int j = 0; j < V; j++) amax = max(amax, __float_as_uint(y[i][j]) & 0x7FFFFFFFu);
             }
@@ -365,7 +358,7 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
         bool odd = false;
         unsure |= amax >= 0x7F800000u;
         const bool all64 = __syncthreads_or(unsure);       // no row's float values are good
-        if (all64 || kv8_exponent(top * (1.f - 2.f * KEY_ERR), I8) != kv8_exponent(top * (1.f + 2.f * KEY_ERR), I8)) {
+        if (all64 || kv8_exponent(top * (1.f - 4.f * KEY_ERR_TURNED), I8) != kv8_exponent(top * (1.f + 4.f * KEY_ERR_TURNED), I8)) {
             uint32_t finite = 0, all = 0;
 #pragma unroll 1
             for (int r = 0; r < mine; r++) {
@@ -384,14 +377,16 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
         settle(amax, odd);
         const float f = kv8_two(-e);
         uint32_t again = 0;                                // rows of which some value's code is not certain
+        const int from = partner<V>(p.rot, lane);
+        const bool turned = lane * V < p.rot;
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
             if (i >= mine) break;
             float a[V], b[V];
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                const float other = __shfl_sync(0xffffffffu, y[i][j], partner<V>(p.rot, lane));
-                const float err = (fabsf(y[i][j]) + fabsf(other)) * KEY_ERR;
+                const float other = __shfl_sync(0xffffffffu, y[i][j], from);
+                const float err = turned ? (fabsf(y[i][j]) + fabsf(other)) * KEY_ERR_TURNED : fabsf(y[i][j]) * KEY_ERR;
                 a[j] = (y[i][j] - err) * f;
                 b[j] = (y[i][j] + err) * f;
             }
@@ -538,7 +533,11 @@ int launch_write_rows(cwk_ctx *ctx, Kv8WriteParams &p, int type) {
     if (PREP) {
         p.heads = p.n * (int64_t)p.B * p.nh <= 16 * 1024 ? 1 : KQ_HEADS;      // query heads that share a token's angles; few rows: one warp each
         blocks += ((int64_t)p.B * p.n * ((p.nh + p.heads - 1) / p.heads) + warps - 1) / warps;
-        smem = (size_t)(p.rot / 2) * warps * sizeof(double2);      // 32 KB at most
+        smem = (size_t)(p.rot / 2) * warps * ROWS * sizeof(float2);      // 128 KB at most (32 KB for 64 values in blocks of 128 rows)
+        static bool attr_set[2][16] = {};
+        bool &set = attr_set[type == CWK_KV8_INT8][ctx->device & 15];
+        if (!set) CWK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 << 10));
+        set = true;
     }
     if (blocks > 0x7FFFFFFF) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "kv8 write: too many rows in one call");
     CWK_CUDA(ctx, cwk_launch_early(kern, dim3((unsigned)blocks), dim3(32 * warps), smem, ctx->stream, p));
