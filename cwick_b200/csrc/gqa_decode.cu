@@ -51,8 +51,12 @@ __global__ void __launch_bounds__(32 * GW) gqa_decode_kernel(const GqaDecodePara
     GqaPlace at{0, 0, 0, 0, 0};
     cwk_pdl_launch();
     cwk_pdl_wait();
-    const int n = gqa_range(p.steps, lane, warp == 0, at);
-    if (n <= 0) return;
+    GqaList list;
+    const int n = gqa_range(p.steps, lane, list, at);
+    if (n <= 0) {
+        if (warp == 0) gqa_note(p.steps, list, lane);
+        return;
+    }
     at.len = length_of(p.steps, at.b);
     GqaPlace ld = at;                                     // the step being loaded
     auto load = [&](int slot) {
@@ -80,6 +84,7 @@ __global__ void __launch_bounds__(32 * GW) gqa_decode_kernel(const GqaDecodePara
         }
         cp_async_commit();
     }
+    if (warp == 0) gqa_note(p.steps, list, lane);
     uint32_t bq[HD / 16][2];                              // the query heads, as the score MMAs' second operand
     float acc[HD / 16][4];                                // value columns 16 i + lg (+ 8) of heads 2 lt, 2 lt + 1
     float m0 = 0.f, m1 = 0.f, l0 = 0.f, l1 = 0.f;

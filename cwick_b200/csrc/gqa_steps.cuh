@@ -21,56 +21,122 @@ struct GqaPlace {
 };
 __device__ __forceinline__ int steps_of(const GqaSteps &p, int b) { return b < p.B ? (length_of(p, b) + p.keys - 1) / p.keys : 0; }
 
-// This block's range [lo, hi) of all steps, and where it begins. Every warp works it out for itself; the first one notes, for
-// every (sequence, head group) whose first step is in the range, its first record slot (slots are numbered by head group
-// plus block: one of the two grows from record to record) and their number.
-__device__ __forceinline__ int gqa_range(const GqaSteps &p, int lane, bool note, GqaPlace &at) {
-    const int nhg = p.groups;
-    int64_t total = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-        int v = steps_of(p, b0 + lane);
+// What a warp knows of the list: its sequence's steps (sequence 32 i + lane), and those up to and with it among the 32; all steps, groups
+// included. One round of up to 32 sequences is kept, more are walked over again: the start of a block is code that runs once, with
+// nothing in flight yet, so what counts is that it is little (divisions in 64 bits, a second walk and the note in front of the first
+// copies were 4 us of a step of 16 sequences).
+struct GqaList {
+    int mine, upto;
+    int64_t total;
+};
+__device__ __forceinline__ void gqa_round(const GqaSteps &p, int b0, int lane, GqaList &s) {
+    s.mine = steps_of(p, b0 + lane);
+    s.upto = s.mine;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        total += v;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, s.upto, o);
+        if (lane >= o) s.upto += u;
     }
-    total *= nhg;
-    const int64_t G = max((int64_t)1, min((int64_t)gridDim.x, total)), g = blockIdx.x;      // no block between two others is left without a step
-    const int64_t lo = g < G ? total * g / G : total, hi = g < G ? total * (g + 1) / G : total;
-    int64_t before = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-        const int mine = steps_of(p, b0 + lane);
-        int v = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += u;
+}
+__device__ __forceinline__ GqaList gqa_list(const GqaSteps &p, int lane) {
+    GqaList s;
+    gqa_round(p, 0, lane, s);
+    s.total = __shfl_sync(0xffffffffu, s.upto, 31);
+    if (p.B > 32) {
+        const int mine = s.mine, upto = s.upto;
+#pragma unroll 1
+        for (int b0 = 32; b0 < p.B; b0 += 32) {
+            gqa_round(p, b0, lane, s);
+            s.total += __shfl_sync(0xffffffffu, s.upto, 31);
         }
-        const int64_t s0 = (before + v - mine) * nhg, s1 = s0 + (int64_t)mine * nhg;       // this lane's sequence: steps [s0, s1)
-        const bool here = mine > 0 && s0 <= lo && lo < s1 && lo < hi;
-        const uint32_t who = __ballot_sync(0xffffffffu, here);
+        s.mine = mine; s.upto = upto;
+    }
+    s.total *= p.groups;
+    return s;
+}
+// body(first sequence of the round, this lane's steps, the steps in front of them, groups included); it is given GqaList's first round
+template <class U, class F>
+__device__ __forceinline__ void gqa_walk(const GqaSteps &p, GqaList s, int lane, F &&body) {
+    U before = 0;
+#pragma unroll 1
+    for (int b0 = 0;;) {
+        body(b0, s.mine, (before + s.upto - s.mine) * (U)p.groups);
+        if ((b0 += 32) >= p.B) return;
+        before += __shfl_sync(0xffffffffu, s.upto, 31);
+        gqa_round(p, b0, lane, s);
+    }
+}
+// The block's range [lo, hi) of `total` steps: all blocks the same number, but for one; no block between two others is left without a step.
+// U: an unsigned type that total * (blocks + 1) fits.
+template <class U> __device__ __forceinline__ U gqa_blocks(U total) { return max((U)1, min((U)gridDim.x, total)); }
+template <class U> __device__ __forceinline__ U gqa_from(U total, U g) {
+    const U G = gqa_blocks(total);
+    return g >= G ? total : G == total ? g : total * g / G;
+}
+template <class U>
+__device__ __forceinline__ int gqa_share(const GqaSteps &p, const GqaList &s, int lane, GqaPlace &at) {
+    const U total = (U)s.total, lo = gqa_from<U>(total, blockIdx.x), hi = gqa_from<U>(total, blockIdx.x + 1);
+    gqa_walk<U>(p, s, lane, [&](int b0, int mine, U s0) {
+        const uint32_t who = __ballot_sync(0xffffffffu, mine > 0 && s0 <= lo && lo < s0 + (U)mine * (U)p.groups && lo < hi);
         if (who) {
             const int src = __ffs(who) - 1;
             at.b = b0 + src;
             at.steps = __shfl_sync(0xffffffffu, mine, src);
-            const int off = (int)__shfl_sync(0xffffffffu, (int)(lo - s0), src);
-            at.hg = off / at.steps;
-            at.step = off % at.steps;
+            const uint32_t off = __shfl_sync(0xffffffffu, (uint32_t)(lo - s0), src);
+            at.hg = p.groups == 1 ? 0 : off / (uint32_t)at.steps;
+            at.step = off - at.hg * at.steps;
         }
-        if (note && b0 + lane < p.B) {
-            if (mine == 0) {
-                if (s0 > 0 ? (lo < s0 && s0 <= hi) : g == 0)
-                    for (int h = 0; h < nhg; h++) p.meta[(b0 + lane) * nhg + h] = make_int2(0, 0);
-            } else if (s0 < hi && s1 > lo) {
-                const int64_t h0 = lo > s0 ? (lo - s0 + mine - 1) / mine : 0;              // first head group that begins here
-                for (int64_t h = h0; h < nhg && s0 + h * mine < hi; h++) {
-                    const int64_t g1 = ((s0 + (h + 1) * mine) * G - 1) / total;              // the block with its last step
-                    p.meta[(b0 + lane) * nhg + h] = make_int2((int)((b0 + lane) * nhg + h + g), (int)(g1 - g + 1));
-                }
+    });
+    return (int)(hi - lo);
+}
+// Where the block begins, and how many steps it has; the list is for gqa_note.
+__device__ __forceinline__ int gqa_range(const GqaSteps &p, int lane, GqaList &s, GqaPlace &at) {
+    if (p.B == 1) {                                        // nothing to add up or to look for
+        s.mine = s.upto = steps_of(p, 0);
+        s.total = (int64_t)s.mine * p.groups;
+        if (s.total * (gridDim.x + 1) < (1ll << 32)) {
+            const uint32_t lo = gqa_from<uint32_t>((uint32_t)s.total, blockIdx.x), hi = gqa_from<uint32_t>((uint32_t)s.total, blockIdx.x + 1);
+            at.steps = s.mine;
+            at.hg = p.groups == 1 || lo == hi ? 0 : lo / (uint32_t)s.mine;
+            at.step = (int)lo - at.hg * s.mine;
+            return (int)(hi - lo);
+        }
+    }
+    s = gqa_list(p, lane);
+    if (s.total * (gridDim.x + 1) < (1ll << 32)) return gqa_share<uint32_t>(p, s, lane, at);
+    return gqa_share<uint64_t>(p, s, lane, at);
+}
+// One warp of the block notes, for every (sequence, head group) whose first step is in the block's range, its first record slot (slots
+// are numbered by head group plus block: one of the two grows from record to record) and their number.
+template <class U>
+__device__ __forceinline__ void gqa_note_as(const GqaSteps &p, const GqaList &s, int lane) {
+    const U total = (U)s.total, nhg = p.groups, G = gqa_blocks(total), g = blockIdx.x, lo = gqa_from<U>(total, g), hi = gqa_from<U>(total, g + 1);
+    gqa_walk<U>(p, s, lane, [&](int b0, int mine, U s0) {
+        const int b = b0 + lane;
+        if (b >= p.B) return;
+        if (mine == 0) {
+            if (s0 > 0 ? (lo < s0 && s0 <= hi) : g == 0)
+                for (int h = 0; h < p.groups; h++) p.meta[b * p.groups + h] = make_int2(0, 0);
+        } else if (s0 < hi && s0 + (U)mine * nhg > lo) {
+            const U h0 = lo > s0 ? (lo - s0 + mine - 1) / (U)mine : 0;                     // first head group that begins here
+#pragma unroll 1
+            for (U h = h0; h < nhg && s0 + h * mine < hi; h++) {
+                const U last = s0 + (h + 1) * mine, g1 = G == total ? last - 1 : (last * G - 1) / total;      // the block with its last step
+                p.meta[b * p.groups + (int)h] = make_int2(b * p.groups + (int)(h + g), (int)(g1 - g + 1));
             }
         }
-        before += __shfl_sync(0xffffffffu, v, 31);
+    });
+}
+__device__ __forceinline__ void gqa_note(const GqaSteps &p, GqaList s, int lane) {
+    if (p.B == 1) {
+        if (p.groups == 1) {
+            if (blockIdx.x == 0 && lane == 0) p.meta[0] = make_int2(0, (int)min((int64_t)gridDim.x, s.total));
+            return;
+        }
+        if (lane > 0) s.mine = 0;                          // (gqa_range may have left the one sequence's steps in every lane)
     }
-    return (int)(hi - lo);
+    if (s.total * (gridDim.x + 1) < (1ll << 32)) gqa_note_as<uint32_t>(p, s, lane);
+    else gqa_note_as<uint64_t>(p, s, lane);
 }
 __device__ __forceinline__ void gqa_advance(const GqaSteps &p, GqaPlace &at) {      // to the next step; there is one
     if (++at.step < at.steps) return;

@@ -31,7 +31,7 @@ struct Kv8DecodeParams {
     int n, nh, nkv, group, hb, lb;    // hb: KV heads a block works on at once (4, 2 or 1); block = 1 << lb
     int per, parts;                   // query tokens whose heads share the MMA columns; parts = ceil(n / per)
     float scale_log2;
-    float *rec;                       // [slot][warp][per * group][hd + 2]
+    float *rec;                       // [slot][warp]: o [per * group][hd], then {m, l} [per * group]
     GqaSteps steps;                   // groups: (nkv / hb) * parts, the parts of the same keys next to each other; keys: GK * (GW / hb)
 };
 
@@ -52,6 +52,9 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// floats of a warp's record: o [cols][HD], {m, l} [cols], a multiple of 16 bytes
+__host__ __device__ __forceinline__ constexpr int kv8_record(int cols, int hd) { return cols * hd + ((2 * cols + 3) & ~3); }
+
 // Places of a warp's ring, each the K or the V of a step: 24 KB a warp, so that two blocks of four warps are on an SM and a scheduler has
 // two of these chains of dependent instructions to choose from.
 template <int HD> constexpr int KV8_RING = HD == 256 ? 3 : 6;
@@ -70,25 +73,46 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
     GqaPlace at{0, 0, 0, 0, 0};
     cwk_pdl_launch();
     cwk_pdl_wait();
-    const int n = gqa_range(p.steps, lane, warp == 0, at);
-    if (n <= 0) return;
+    GqaList list;
+    const int n = gqa_range(p.steps, lane, list, at);
+    if (n <= 0) {
+        if (warp == 0) gqa_note(p.steps, list, lane);
+        return;
+    }
     at.len = length_of(p.steps, at.b);
     GqaPlace ld = at;                                     // the step being loaded
     auto head_of = [&](const GqaPlace &x) { return (x.hg / p.parts) * p.hb + wh; };
+    auto query = [&](const GqaPlace &x, int col, bool &on) {      // row `col` of the place's queries
+        const int tok = x.hg % p.parts * p.per + col / p.group;
+        on = col < cols && tok < p.n;
+        return p.q + (((int64_t)x.b * p.n + tok) * p.nh + head_of(x) * p.group + col % p.group) * HD;
+    };
+    {   // on their way while the first copies are asked for
+        bool on;
+        const uint16_t *qr = query(at, lane / (HD / 64), on) + lane % (HD / 64) * 64;
+        if (on) asm volatile("prefetch.global.L1 [%0];" ::"l"(qr));
+    }
     int halves = 2 * n, ld_place = 0;                     // halves of steps (K, then V) still to be asked for; the place of the next one
+    const int64_t row = (int64_t)p.nkv * HD;
+    const int ld_c = lane % CH, ld_r = lane / CH;         // this lane's piece of a row, and which of the rows that one instruction copies
+    int64_t ld_at = 0;                                    // where they are, for the step being loaded
     auto load_next = [&]() {
         if (halves > 0) {
-            const int j0 = ld.step * keys + sub * GK;
-            const int64_t row = (int64_t)p.nkv * HD;
-            const uint8_t *src = ((halves & 1) ? p.v : p.k) + (int64_t)ld.b * p.rows * row + head_of(ld) * HD;
-            const uint32_t dst = ring + ld_place * KB;
             constexpr int RPI = 32 / CH;                  // rows per instruction: 2 or 4
-            const int c = lane % CH, rr = lane / CH;
+            const int j0 = ld.step * keys + sub * GK;
+            if (!(halves & 1)) ld_at = ((int64_t)ld.b * p.rows + j0 + ld_r) * row + head_of(ld) * HD + ld_c * 16;
+            const uint8_t *src = ((halves & 1) ? p.v : p.k) + ld_at;
+            const uint32_t dst = ring + ld_place * KB + ld_r * HD;
+            if (j0 + GK <= ld.len) {
 #pragma unroll
-            for (int i = 0; i < GK / RPI; i++) {
-                const int r = i * RPI + rr;
-                const bool ok = j0 + r < ld.len;          // (rows behind the last are not read: zeros in their place)
-                cp_async16(dst + r * HD + ((c ^ (r & 7)) << 4), src + (ok ? (int64_t)(j0 + r) * row : 0) + c * 16, ok);
+                for (int i = 0; i < GK / RPI; i++, src += RPI * row)
+                    cp_async16(dst + i * RPI * HD + ((ld_c ^ ((i * RPI + ld_r) & 7)) << 4), src, true);
+            } else {                                      // (rows behind the last are not read: zeros in their place)
+#pragma unroll
+                for (int i = 0; i < GK / RPI; i++, src += RPI * row) {
+                    const bool ok = j0 + i * RPI + ld_r < ld.len;
+                    cp_async16(dst + i * RPI * HD + ((ld_c ^ ((i * RPI + ld_r) & 7)) << 4), ok ? src : p.k, ok);
+                }
             }
             halves--;
             ld_place = ld_place + 1 == RING ? 0 : ld_place + 1;
@@ -96,20 +120,24 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
         }
         cp_async_commit();
     };
-    // the two scales of this warp's keys at a place (any value where it has no key there)
-    auto scales = [&](const GqaPlace &x) -> uint32_t {
+    // the two scales of this warp's keys at a place (any value where it has no key there), not joined: that would wait for them
+    auto scales = [&](const GqaPlace &x, uint32_t &ks, uint32_t &vs) {
         const int j0 = x.step * keys + sub * GK;
-        if (j0 >= x.len) return 127u | 127u << 8;
+        ks = vs = 127;
+        if (j0 >= x.len) return;
         const int64_t i = ((int64_t)x.b * (p.rows >> p.lb) + (j0 >> p.lb)) * p.nkv + head_of(x);
-        return (uint32_t)p.ks[i] | (uint32_t)p.vs[i] << 8;
+        ks = p.ks[i];
+        vs = p.vs[i];
     };
+    uint32_t ks, vs;
+    scales(at, ks, vs);
 #pragma unroll
     for (int i = 0; i < RING - 1; i++) load_next();
+    if (warp == 0) gqa_note(p.steps, list, lane);
     uint32_t bq[HD / 16][NB][2];                          // the query rows, as the score MMAs' second operand
     float acc[HD / 16][NB][4];                            // value columns 16 i + 2 lg (+ 1) of query rows 8 nb + 2 lt, + 1
     float m[NB][2], l[NB][2], unit[NB][2];                // unit: what a score MMA's result is multiplied by, besides the key scale
     int limit[NB][2];                                     // rows that the query row sees
-    uint32_t sc = scales(at);
     bool fresh = true;
     int place = 0;                                        // of the half in use
     for (int s = 0; s < n; s++) {
@@ -118,17 +146,18 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
                 // this lane's dims of query row 8 nb + lg: 16 i + 4 lt .. + 3
-                const int col = nb * 8 + lg, tok = part * p.per + col / p.group;
-                const bool on = col < cols && tok < p.n;
-                const uint16_t *qr = p.q + (((int64_t)at.b * p.n + tok) * p.nh + head_of(at) * p.group + col % p.group) * HD + 4 * lt;
+                bool on;
+                const uint16_t *qr = query(at, nb * 8 + lg, on) + 4 * lt;
                 uint2 u[HD / 16];
-                float big = 0.f;
+                __nv_bfloat162 top = __float2bfloat162_rn(0.f);
+#pragma unroll
+                for (int i = 0; i < HD / 16; i++) u[i] = on ? *reinterpret_cast<const uint2 *>(qr + i * 16) : make_uint2(0u, 0u);
 #pragma unroll
                 for (int i = 0; i < HD / 16; i++) {
-                    u[i] = on ? *reinterpret_cast<const uint2 *>(qr + i * 16) : make_uint2(0u, 0u);
-                    big = fmaxf(fmaxf(big, fmaxf(fabsf(__uint_as_float(u[i].x << 16)), fabsf(__uint_as_float(u[i].x & 0xFFFF0000u)))),
-                                fmaxf(fabsf(__uint_as_float(u[i].y << 16)), fabsf(__uint_as_float(u[i].y & 0xFFFF0000u))));
+                    top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&u[i].x)));
+                    top = __hmax2(top, __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&u[i].y)));
                 }
+                float big = fmaxf(__low2float(top), __high2float(top));
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
                 big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
                 const int e = min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 120);
@@ -153,20 +182,20 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
         __syncwarp();                                     // every lane's copies of these keys have landed; the place before has been read
         load_next();
         GqaPlace next = at;                               // its scales are asked for a step ahead
-        uint32_t sc_next = 0;
+        uint32_t ks_next = 0, vs_next = 0;
         if (s + 1 < n) {
             gqa_advance(p.steps, next);
-            sc_next = scales(next);
+            scales(next, ks_next, vs_next);
         }
         const uint32_t tK = ring + place * KB;
         place = place + 1 == RING ? 0 : place + 1;
-        const uint32_t row = lane * HD, x7 = lane & 7;    // ldmatrix: a lane's address is key `lane`'s
-        const float kscale = kv8_scale(sc & 255u), vscale = kv8_scale(sc >> 8);
+        const uint32_t key = lane * HD, x7 = lane & 7;    // ldmatrix: a lane's address is key `lane`'s
+        const float kscale = kv8_scale(ks), vscale = kv8_scale(vs);
         float c[2][NB][4];                                // scores of keys 16 h + lg, + 8
 #pragma unroll
         for (int i = 0; i < HD / 16; i++) {
             uint32_t r[4], a[2][4];
-            ldmatrix_x4(r[0], r[1], r[2], r[3], tK + row + ((i ^ x7) << 4));
+            ldmatrix_x4(r[0], r[1], r[2], r[3], tK + key + ((i ^ x7) << 4));
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 kv8_decode4<I8>(r[2 * h], a[h][0], a[h][2]);
@@ -233,7 +262,7 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
 #pragma unroll
         for (int i = 0; i < HD / 16; i++) {
             uint32_t r[4], a[2][4];
-            ldmatrix_x4_trans(r[0], r[1], r[2], r[3], tV + row + ((i ^ x7) << 4));
+            ldmatrix_x4_trans(r[0], r[1], r[2], r[3], tV + key + ((i ^ x7) << 4));
             float d[NB][4];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -253,7 +282,7 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
         fresh = at.step + 1 == at.steps;
         if (fresh || s + 1 == n) {                        // the end of what this block has of the sequence's head group: its record
             const int64_t slot = (int64_t)at.b * p.steps.groups + at.hg + blockIdx.x;
-            float *rec = p.rec + (slot * GW + warp) * cols * (HD + 2);
+            float *rec = p.rec + (slot * GW + warp) * kv8_record(cols, HD);
 #pragma unroll
             for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -263,35 +292,79 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
                     for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                     const int col = nb * 8 + 2 * lt + x;
                     if (col >= cols) continue;
-                    float *o = rec + col * (HD + 2);
-                    if (lg == 0) *reinterpret_cast<float2 *>(o) = make_float2(sum != 0.f ? m[nb][x] : -INFINITY, sum);
+                    float *o = rec + col * HD;
+                    if (lg == 0) *reinterpret_cast<float2 *>(rec + cols * HD + col * 2) = make_float2(sum != 0.f ? m[nb][x] : -INFINITY, sum);
 #pragma unroll
                     for (int i = 0; i < HD / 16; i++)
-                        *reinterpret_cast<float2 *>(o + 2 + i * 16 + 2 * lg) = make_float2(acc[i][nb][x], acc[i][nb][2 + x]);
+                        *reinterpret_cast<float2 *>(o + i * 16 + 2 * lg) = make_float2(acc[i][nb][x], acc[i][nb][2 + x]);
                 }
         }
         at = next;
-        sc = sc_next;
+        ks = ks_next; vs = vs_next;
     }
     cp_async_wait<0>();
 }
 
-// grid (query row = token x head, sequence), (HD / 2) x GROUPS threads (gqa_merge_records)
+// grid (query row = token x head, sequence, 64 of its columns), 16 x GROUPS threads: four columns each, the records dealt out to the groups.
+// (One sequence has a record from every block: what counts is that all of them are asked for at once.)
 template <int HD, int GROUPS>
-__global__ void __launch_bounds__(HD / 2 * GROUPS) kv8_merge_kernel(const Kv8DecodeParams p, uint16_t *out) {
+__global__ void __launch_bounds__(16 * GROUPS) kv8_merge_kernel(const Kv8DecodeParams p, uint16_t *out) {
+    __shared__ float s_m[GROUPS], s_l[GROUPS];
+    __shared__ float4 s_o[GROUPS][16];
     const int tok = blockIdx.x / p.nh, h = blockIdx.x % p.nh, b = blockIdx.y, kvh = h / p.group, ks = GW / p.hb, cols = p.per * p.group;
-    const int tid = threadIdx.x % (HD / 2);
+    const int g = threadIdx.x / 16, t = threadIdx.x % 16, at = blockIdx.z * 64 + t * 4;
     cwk_pdl_launch();
     cwk_pdl_wait();
     const int2 meta = p.steps.meta[b * p.steps.groups + (kvh / p.hb) * p.parts + tok / p.per];
-    const int64_t rsz = (int64_t)cols * (HD + 2);
+    const int64_t rsz = kv8_record(cols, HD);
+    const int col = tok % p.per * p.group + h % p.group, cnt = meta.y * ks;
     // record i: slot first + i / ks, warp (i % ks) * hb + kvh % hb
-    const float *base = p.rec + ((int64_t)meta.x * GW + kvh % p.hb) * rsz + (int64_t)((tok % p.per) * p.group + h % p.group) * (HD + 2);
-    auto at = [&](int i) { return base + (ks == 1 ? (int64_t)i * GW : (int64_t)(i / ks) * GW + (i % ks) * p.hb) * rsz; };
-    float den, x, y;
-    if (!gqa_merge_records<HD, GROUPS>(meta.y * ks, at, den, x, y)) return;
+    const float *base = p.rec + ((int64_t)meta.x * GW + kvh % p.hb) * rsz;
+    float M = -INFINITY, den = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i0 = g; i0 < cnt; i0 += 8 * GROUPS) {         // eight records' loads at once; the running maximum as the scores'
+        float2 ml[8];
+        float4 o[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int i = min(i0 + j * GROUPS, cnt - 1);
+            const float *r = base + (ks == 1 ? (int64_t)i * GW : (int64_t)(i / ks) * GW + (i % ks) * p.hb) * rsz;
+            ml[j] = *reinterpret_cast<const float2 *>(r + cols * HD + col * 2);
+            o[j] = *reinterpret_cast<const float4 *>(r + col * HD + at);
+            if (i0 + j * GROUPS >= cnt) ml[j].x = -INFINITY;
+        }
+        float mx = M;
+#pragma unroll
+        for (int j = 0; j < 8; j++) mx = fmaxf(mx, ml[j].x);
+        if (mx == -INFINITY) continue;
+        const float a = exp2f(M - mx);
+        den *= a; sum.x *= a; sum.y *= a; sum.z *= a; sum.w *= a;
+        M = mx;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float w = exp2f(ml[j].x - M);
+            den += w * ml[j].y; sum.x += w * o[j].x; sum.y += w * o[j].y; sum.z += w * o[j].z; sum.w += w * o[j].w;
+        }
+    }
+    if (GROUPS > 1) {
+        if (t == 0) { s_m[g] = M; s_l[g] = den; }
+        s_o[g][t] = sum;
+        __syncthreads();
+        if (g > 0) return;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < GROUPS; j++) mx = fmaxf(mx, s_m[j]);
+        den = 0.f;
+        sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < GROUPS; j++) {
+            const float w = s_m[j] == -INFINITY ? 0.f : exp2f(s_m[j] - mx);
+            const float4 o = s_o[j][t];
+            den += w * s_l[j]; sum.x += w * o.x; sum.y += w * o.y; sum.z += w * o.z; sum.w += w * o.w;
+        }
+    }
     const float inv = den != 0.f ? 1.f / den : 0.f;
-    *reinterpret_cast<uint32_t *>(out + (((int64_t)b * p.n + tok) * p.nh + h) * HD + 2 * tid) = pack_bf16x2(x * inv, y * inv);
+    *reinterpret_cast<uint2 *>(out + (((int64_t)b * p.n + tok) * p.nh + h) * HD + at) = make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
 }
 
 template <int HD, int NB>
@@ -309,9 +382,10 @@ int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *o
         CWK_CUDA(ctx, cwk_launch_early(kern, dim3(blocks), dim3(32 * GW), SMEM, ctx->stream, p));
         ctx->launches++;
     }
-    const bool many = (int64_t)blocks * (GW / p.hb) > 8 * (int64_t)p.steps.B * p.parts;      // records per query row
-    CWK_CUDA(ctx, cwk_launch_early(many ? kv8_merge_kernel<HD, 8> : kv8_merge_kernel<HD, 1>, dim3(p.n * p.nh, p.steps.B), dim3(HD / 2 * (many ? 8 : 1)), 0,
-                                   ctx->stream, p, (uint16_t *)out));
+    // records per query row: more than eight, or a group's loads suffice
+    const int64_t each = (int64_t)blocks * (GW / p.hb) / ((int64_t)p.steps.B * p.parts);
+    CWK_CUDA(ctx, cwk_launch_early(each > 32 ? kv8_merge_kernel<HD, 16> : each > 8 ? kv8_merge_kernel<HD, 8> : kv8_merge_kernel<HD, 2>,
+                                   dim3(p.n * p.nh, p.steps.B, HD / 64), dim3(each > 32 ? 256 : each > 8 ? 128 : 32), 0, ctx->stream, p, (uint16_t *)out));
     ctx->launches++;
     return CWK_OK;
 }
@@ -332,7 +406,7 @@ int cwk_kv8_streams(cwk_ctx *ctx, const void *q, const cwk_kv8 &c, const int32_t
     const int64_t groups = (int64_t)(c.nkv / p.hb) * p.parts;
     const int64_t most = std::max<int64_t>(1, B * groups * ((max_kv_len + keys - 1) / keys));
     const int blocks = (int)std::min<int64_t>(most, max_blocks > 0 ? std::min(max_blocks, 2 * ctx->sm_count) : 2 * ctx->sm_count);
-    const size_t rec_bytes = (size_t)(B * groups + blocks) * GW * p.per * p.group * (c.hd + 2) * sizeof(float);
+    const size_t rec_bytes = (size_t)(B * groups + blocks) * GW * kv8_record(p.per * p.group, c.hd) * sizeof(float);
     const int s = cwk_reserve_scratch(ctx, rec_bytes + (size_t)B * groups * sizeof(int2));
     if (s != CWK_OK) return s;
     p.rec = ctx->scratch;
