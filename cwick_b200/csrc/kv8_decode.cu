@@ -56,18 +56,23 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 __host__ __device__ __forceinline__ constexpr int kv8_record(int cols, int hd) { return cols * hd + ((2 * cols + 3) & ~3); }
 
 // Places of a warp's ring, each the K or the V of a step: 24 KB a warp, so that two blocks of four warps are on an SM and a scheduler has
-// two of these chains of dependent instructions to choose from.
-template <int HD> constexpr int KV8_RING = HD == 256 ? 3 : 6;
+// two of these chains of dependent instructions to choose from. Sixteen query rows of 256 leave no registers for the query fragments
+// beside the accumulators: they take the third place of the ring (4 tokens of 64 sequences of 4096 rows 124 -> 107 us).
+template <int HD, int NB> constexpr bool KV8_Q_SHARED = HD == 256 && NB == 2;
+template <int HD, int NB> constexpr int KV8_RING = KV8_Q_SHARED<HD, NB> ? 2 : HD == 256 ? 3 : 6;
 
 // NB: groups of eight MMA columns (query rows)
 template <int HD, int NB, bool I8>
 __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeParams p) {
     constexpr int CH = HD / 16;                           // 16-byte pieces per row
-    constexpr int RING = KV8_RING<HD>;
+    constexpr int RING = KV8_RING<HD, NB>;
+    constexpr bool QS = KV8_Q_SHARED<HD, NB>;
     constexpr int KB = GK * HD;                           // bytes of a place of the ring
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lg = lane >> 2, lt = lane & 3;
-    const uint32_t ring = smem_u32(smem) + warp * RING * KB;
+    const uint32_t ring = smem_u32(smem) + warp * (RING + (QS ? 1 : 0)) * KB;
+    uint4 *qs = reinterpret_cast<uint4 *>(smem + (warp * (RING + 1) + RING) * KB) + lane;      // QS: [HD / 16][lane]
+    static_assert(!QS || HD / 16 * 32 * 16 <= KB, "query fragments");
     const int sub = warp / p.hb, wh = warp % p.hb;        // which 32 keys of a step, which KV head of the group
     const int keys = p.steps.keys, cols = p.per * p.group;
     GqaPlace at{0, 0, 0, 0, 0};
@@ -134,7 +139,7 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
 #pragma unroll
     for (int i = 0; i < RING - 1; i++) load_next();
     if (warp == 0) gqa_note(p.steps, list, lane);
-    uint32_t bq[HD / 16][NB][2];                          // the query rows, as the score MMAs' second operand
+    uint32_t bq[QS ? 1 : HD / 16][NB][2];                 // the query rows, as the score MMAs' second operand
     float acc[HD / 16][NB][4];                            // value columns 16 i + 2 lg (+ 1) of query rows 8 nb + 2 lt, + 1
     float m[NB][2], l[NB][2], unit[NB][2];                // unit: what a score MMA's result is multiplied by, besides the key scale
     int limit[NB][2];                                     // rows that the query row sees
@@ -164,8 +169,10 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
                 const float down = kv8_two(-e);
 #pragma unroll
                 for (int i = 0; i < HD / 16; i++) {
-                    bq[i][nb][0] = pack_f16x2(__uint_as_float(u[i].x << 16) * down, __uint_as_float(u[i].x & 0xFFFF0000u) * down);
-                    bq[i][nb][1] = pack_f16x2(__uint_as_float(u[i].y << 16) * down, __uint_as_float(u[i].y & 0xFFFF0000u) * down);
+                    const uint32_t q0 = pack_f16x2(__uint_as_float(u[i].x << 16) * down, __uint_as_float(u[i].x & 0xFFFF0000u) * down);
+                    const uint32_t q1 = pack_f16x2(__uint_as_float(u[i].y << 16) * down, __uint_as_float(u[i].y & 0xFFFF0000u) * down);
+                    if constexpr (QS) reinterpret_cast<uint2 *>(qs + i * 32)[nb] = make_uint2(q0, q1);      // (read by this lane alone)
+                    else { bq[i][nb][0] = q0; bq[i][nb][1] = q1; }
                     acc[i][nb][0] = acc[i][nb][1] = acc[i][nb][2] = acc[i][nb][3] = 0.f;
                 }
                 // the two rows whose scores this lane gets are those of lanes with lg = 2 lt, 2 lt + 1
@@ -196,14 +203,22 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
         for (int i = 0; i < HD / 16; i++) {
             uint32_t r[4], a[2][4];
             ldmatrix_x4(r[0], r[1], r[2], r[3], tK + key + ((i ^ x7) << 4));
+            uint32_t q[NB][2];
+            if constexpr (QS) {
+                const uint4 v = qs[i * 32];
+                q[0][0] = v.x; q[0][1] = v.y; q[NB - 1][0] = v.z; q[NB - 1][1] = v.w;
+            } else {
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) { q[nb][0] = bq[i][nb][0]; q[nb][1] = bq[i][nb][1]; }
+            }
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 kv8_decode4<I8>(r[2 * h], a[h][0], a[h][2]);
                 kv8_decode4<I8>(r[2 * h + 1], a[h][1], a[h][3]);
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++) {
-                    if (i == 0) mma_f16_16816_zero(c[h][nb], a[h], bq[i][nb][0], bq[i][nb][1]);
-                    else mma_f16_16816(c[h][nb], a[h], bq[i][nb][0], bq[i][nb][1]);
+                    if (i == 0) mma_f16_16816_zero(c[h][nb], a[h], q[nb][0], q[nb][1]);
+                    else mma_f16_16816(c[h][nb], a[h], q[nb][0], q[nb][1]);
                 }
             }
         }
@@ -305,71 +320,94 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
     cp_async_wait<0>();
 }
 
-// grid (query row = token x head, sequence, 64 of its columns), 16 x GROUPS threads: four columns each, the records dealt out to the groups.
-// (One sequence has a record from every block: what counts is that all of them are asked for at once.)
+// The records of one query row (token x head of sequence b): cnt of them, {m, l} and o of the i-th at ml(i) and o(i).
+struct Kv8Records {
+    const float *base;
+    int64_t rsz;
+    int cnt, ks, hb, ml, o;
+    __device__ __forceinline__ Kv8Records(const Kv8DecodeParams &p, int hd, int b, int tok, int h) {
+        const int kvh = h / p.group, cols = p.per * p.group, col = tok % p.per * p.group + h % p.group;
+        const int2 meta = p.steps.meta[b * p.steps.groups + (kvh / p.hb) * p.parts + tok / p.per];
+        hb = p.hb; ks = GW / hb; cnt = meta.y * ks;
+        rsz = kv8_record(cols, hd);
+        ml = cols * hd + col * 2; o = col * hd;
+        base = p.rec + ((int64_t)meta.x * GW + kvh % hb) * rsz;
+    }
+    // slot first + i / ks, warp (i % ks) * hb + kvh % hb
+    __device__ __forceinline__ const float *at(int i) const { return base + (ks == 1 ? (int64_t)i * GW : (int64_t)(i / ks) * GW + (i % ks) * hb) * rsz; }
+};
+// Four columns of the records first, first + stride, .., eight records' loads at once; the running maximum as the scores'.
+struct Kv8Sum {
+    float M = -INFINITY, den = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    __device__ __forceinline__ void add(float w, float l, const float4 &v) {
+        den += w * l; o.x += w * v.x; o.y += w * v.y; o.z += w * v.z; o.w += w * v.w;
+    }
+    __device__ __forceinline__ void run(const Kv8Records &r, int column, int first, int stride) {
+        for (int i0 = first; i0 < r.cnt; i0 += 8 * stride) {
+            float2 ml[8];
+            float4 v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float *at = r.at(min(i0 + j * stride, r.cnt - 1));
+                ml[j] = *reinterpret_cast<const float2 *>(at + r.ml);
+                v[j] = *reinterpret_cast<const float4 *>(at + r.o + column);
+                if (i0 + j * stride >= r.cnt) ml[j].x = -INFINITY;
+            }
+            float to = M;
+#pragma unroll
+            for (int j = 0; j < 8; j++) to = fmaxf(to, ml[j].x);
+            if (to == -INFINITY) continue;
+            const float a = exp2f(M - to);
+            den *= a; o.x *= a; o.y *= a; o.z *= a; o.w *= a;
+            M = to;
+#pragma unroll
+            for (int j = 0; j < 8; j++) add(exp2f(ml[j].x - M), ml[j].y, v[j]);
+        }
+    }
+    __device__ __forceinline__ void write(uint16_t *out) const {
+        const float inv = den != 0.f ? 1.f / den : 0.f;
+        *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    }
+};
+
+// Few records a row: 256 threads have the rows of a sequence one after another, four columns each. grid (parts of n * nh rows, sequence)
+template <int HD>
+__global__ void __launch_bounds__(256) kv8_merge_few_kernel(const Kv8DecodeParams p, uint16_t *out) {
+    const int row = blockIdx.x * (1024 / HD) + threadIdx.x / (HD / 4), column = threadIdx.x % (HD / 4) * 4, b = blockIdx.y;
+    cwk_pdl_launch();
+    cwk_pdl_wait();
+    if (row >= p.n * p.nh) return;
+    Kv8Sum s;
+    s.run(Kv8Records(p, HD, b, row / p.nh, row % p.nh), column, 0, 1);
+    s.write(out + ((int64_t)b * p.n * p.nh + row) * HD + column);
+}
+// Many: 64 columns of a row to a block, its records dealt out to GROUPS groups of 16 threads: what counts is that all are asked for at
+// once. grid (row, sequence, HD / 64)
 template <int HD, int GROUPS>
 __global__ void __launch_bounds__(16 * GROUPS) kv8_merge_kernel(const Kv8DecodeParams p, uint16_t *out) {
     __shared__ float s_m[GROUPS], s_l[GROUPS];
     __shared__ float4 s_o[GROUPS][16];
-    const int tok = blockIdx.x / p.nh, h = blockIdx.x % p.nh, b = blockIdx.y, kvh = h / p.group, ks = GW / p.hb, cols = p.per * p.group;
-    const int g = threadIdx.x / 16, t = threadIdx.x % 16, at = blockIdx.z * 64 + t * 4;
+    const int row = blockIdx.x, b = blockIdx.y, g = threadIdx.x / 16, t = threadIdx.x % 16, column = blockIdx.z * 64 + t * 4;
     cwk_pdl_launch();
     cwk_pdl_wait();
-    const int2 meta = p.steps.meta[b * p.steps.groups + (kvh / p.hb) * p.parts + tok / p.per];
-    const int64_t rsz = kv8_record(cols, HD);
-    const int col = tok % p.per * p.group + h % p.group, cnt = meta.y * ks;
-    // record i: slot first + i / ks, warp (i % ks) * hb + kvh % hb
-    const float *base = p.rec + ((int64_t)meta.x * GW + kvh % p.hb) * rsz;
-    float M = -INFINITY, den = 0.f;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i0 = g; i0 < cnt; i0 += 8 * GROUPS) {         // eight records' loads at once; the running maximum as the scores'
-        float2 ml[8];
-        float4 o[8];
+    Kv8Sum s;
+    s.run(Kv8Records(p, HD, b, row / p.nh, row % p.nh), column, g, GROUPS);
+    if (t == 0) { s_m[g] = s.M; s_l[g] = s.den; }
+    s_o[g][t] = s.o;
+    __syncthreads();
+    if (g > 0) return;
+    Kv8Sum all;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int i = min(i0 + j * GROUPS, cnt - 1);
-            const float *r = base + (ks == 1 ? (int64_t)i * GW : (int64_t)(i / ks) * GW + (i % ks) * p.hb) * rsz;
-            ml[j] = *reinterpret_cast<const float2 *>(r + cols * HD + col * 2);
-            o[j] = *reinterpret_cast<const float4 *>(r + col * HD + at);
-            if (i0 + j * GROUPS >= cnt) ml[j].x = -INFINITY;
-        }
-        float mx = M;
+    for (int j = 0; j < GROUPS; j++) all.M = fmaxf(all.M, s_m[j]);
 #pragma unroll
-        for (int j = 0; j < 8; j++) mx = fmaxf(mx, ml[j].x);
-        if (mx == -INFINITY) continue;
-        const float a = exp2f(M - mx);
-        den *= a; sum.x *= a; sum.y *= a; sum.z *= a; sum.w *= a;
-        M = mx;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float w = exp2f(ml[j].x - M);
-            den += w * ml[j].y; sum.x += w * o[j].x; sum.y += w * o[j].y; sum.z += w * o[j].z; sum.w += w * o[j].w;
-        }
-    }
-    if (GROUPS > 1) {
-        if (t == 0) { s_m[g] = M; s_l[g] = den; }
-        s_o[g][t] = sum;
-        __syncthreads();
-        if (g > 0) return;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < GROUPS; j++) mx = fmaxf(mx, s_m[j]);
-        den = 0.f;
-        sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int j = 0; j < GROUPS; j++) {
-            const float w = s_m[j] == -INFINITY ? 0.f : exp2f(s_m[j] - mx);
-            const float4 o = s_o[j][t];
-            den += w * s_l[j]; sum.x += w * o.x; sum.y += w * o.y; sum.z += w * o.z; sum.w += w * o.w;
-        }
-    }
-    const float inv = den != 0.f ? 1.f / den : 0.f;
-    *reinterpret_cast<uint2 *>(out + (((int64_t)b * p.n + tok) * p.nh + h) * HD + at) = make_uint2(pack_bf16x2(sum.x * inv, sum.y * inv), pack_bf16x2(sum.z * inv, sum.w * inv));
+    for (int j = 0; j < GROUPS; j++) all.add(s_m[j] == -INFINITY ? 0.f : exp2f(s_m[j] - all.M), s_l[j], s_o[j][t]);
+    all.write(out + ((int64_t)b * p.n * p.nh + row) * HD + column);
 }
 
 template <int HD, int NB>
 int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *out) {
-    constexpr int SMEM = GW * KV8_RING<HD> * GK * HD;      // 96 KB
+    constexpr int SMEM = GW * (KV8_RING<HD, NB> + (KV8_Q_SHARED<HD, NB> ? 1 : 0)) * GK * HD;      // 96 KB
     const bool i8 = type == CWK_KV8_INT8;
     auto kern = i8 ? kv8_decode_kernel<HD, NB, true> : kv8_decode_kernel<HD, NB, false>;
     static bool attr_set[2][16] = {};
@@ -382,10 +420,11 @@ int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *o
         CWK_CUDA(ctx, cwk_launch_early(kern, dim3(blocks), dim3(32 * GW), SMEM, ctx->stream, p));
         ctx->launches++;
     }
-    // records per query row: more than eight, or a group's loads suffice
-    const int64_t each = (int64_t)blocks * (GW / p.hb) / ((int64_t)p.steps.B * p.parts);
-    CWK_CUDA(ctx, cwk_launch_early(each > 32 ? kv8_merge_kernel<HD, 16> : each > 8 ? kv8_merge_kernel<HD, 8> : kv8_merge_kernel<HD, 2>,
-                                   dim3(p.n * p.nh, p.steps.B, HD / 64), dim3(each > 32 ? 256 : each > 8 ? 128 : 32), 0, ctx->stream, p, (uint16_t *)out));
+    const int64_t each = (int64_t)blocks * (GW / p.hb) / ((int64_t)p.steps.B * p.parts);      // records per query row
+    const int rows = p.n * p.nh;
+    if (each > 8) CWK_CUDA(ctx, cwk_launch_early(each > 32 ? kv8_merge_kernel<HD, 16> : kv8_merge_kernel<HD, 8>, dim3(rows, p.steps.B, HD / 64),
+                                                 dim3(each > 32 ? 256 : 128), 0, ctx->stream, p, (uint16_t *)out));
+    else CWK_CUDA(ctx, cwk_launch_early(kv8_merge_few_kernel<HD>, dim3((rows + 1024 / HD - 1) / (1024 / HD), p.steps.B), dim3(256), 0, ctx->stream, p, (uint16_t *)out));
     ctx->launches++;
     return CWK_OK;
 }
