@@ -422,8 +422,9 @@ int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *o
     }
     const int64_t each = (int64_t)blocks * (GW / p.hb) / ((int64_t)p.steps.B * p.parts);      // records per query row
     const int rows = p.n * p.nh;
-    if (each > 8) CWK_CUDA(ctx, cwk_launch_early(each > 32 ? kv8_merge_kernel<HD, 16> : kv8_merge_kernel<HD, 8>, dim3(rows, p.steps.B, HD / 64),
-                                                 dim3(each > 32 ? 256 : 128), 0, ctx->stream, p, (uint16_t *)out));
+    const int groups = each > 32 && (int64_t)rows * p.steps.B * (HD / 64) <= 512 ? 16 : 8;
+    if (each > 8) CWK_CUDA(ctx, cwk_launch_early(groups == 16 ? kv8_merge_kernel<HD, 16> : kv8_merge_kernel<HD, 8>, dim3(rows, p.steps.B, HD / 64),
+                                                 dim3(16 * groups), 0, ctx->stream, p, (uint16_t *)out));
     else CWK_CUDA(ctx, cwk_launch_early(kv8_merge_few_kernel<HD>, dim3((rows + 1024 / HD - 1) / (1024 / HD), p.steps.B), dim3(256), 0, ctx->stream, p, (uint16_t *)out));
     ctx->launches++;
     return CWK_OK;
