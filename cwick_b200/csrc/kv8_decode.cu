@@ -455,6 +455,10 @@ int cwk_kv8_streams(cwk_ctx *ctx, const void *q, const cwk_kv8 &c, const int32_t
     return c.hd == 256 ? launch<256, 1>(ctx, p, c.type, blocks, out) : launch<128, 1>(ctx, p, c.type, blocks, out);
 }
 
+// mla_prefill_attn.cu
+int cwk_gqa_prefill_tc(cwk_ctx *ctx, const void *Q, const void *K, const void *V, int64_t pos, int n, int nh, int nkv, int hd,
+                       float scale, void *out, int *flags);
+
 extern "C" {
 
 int cwk_gqa_decode_kv8(cwk_ctx *ctx, const void *q, const cwk_kv8 *c, const int32_t *kv_len, int max_kv_len, int B, int n, int nh, float scale,
@@ -477,11 +481,9 @@ int cwk_gqa_prefill_kv8(cwk_ctx *ctx, const void *Q, const cwk_kv8 *c, int slot,
     if (!ctx || !Q || !out) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_prefill_kv8: null argument");
     if (slot < 0 || slot >= c->slots || n <= 0 || pos < 0 || pos > c->rows - n || nh <= 0 || nh % c->nkv != 0)
         return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_prefill_kv8: bad dimensions");
-    const int group = nh / c->nkv;
-    if (group > 16 || 64 % group != 0) return cwk_fail(ctx, CWK_ERR_UNSUPPORTED, "gqa_prefill_kv8: group %d not built (1, 2, 4, 8, 16)", group);
     if ((((uintptr_t)Q | (uintptr_t)out) & 15) != 0) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_prefill_kv8: pointers must be 16-byte aligned");
     CWK_CUDA(ctx, cudaSetDevice(ctx->device));
-    // the slot's rows widened, exactly, behind the flags that the bf16 kernel keeps at the start of the workspace
+    // the slot's rows widened, exactly, behind the flags that the bf16 kernel keeps at the start of the workspace (a word per item and SM)
     cwk_kv8 at = *c;
     const int64_t T = pos + n, row = (int64_t)c->nkv * c->hd;
     at.k = (uint8_t *)c->k + slot * c->rows * row; at.v = (uint8_t *)c->v + slot * c->rows * row;
@@ -492,7 +494,8 @@ int cwk_gqa_prefill_kv8(cwk_ctx *ctx, const void *Q, const cwk_kv8 *c, int slot,
     uint8_t *wk = (uint8_t *)ctx->work + flags;
     s = cwk_kv8_widen(ctx, at, 0, T, wk, wk + half);
     if (s != CWK_OK) return s;
-    return cwk_gqa_prefill(ctx, Q, wk, wk + half, pos, n, nh, c->nkv, c->hd, scale, out);
+    s = cwk_gqa_prefill_tc(ctx, Q, wk, wk + half, pos, n, nh, c->nkv, c->hd, scale, out, (int *)ctx->work);
+    return s == CWK_ERR_UNSUPPORTED ? cwk_fail(ctx, s, "gqa_prefill_kv8: tensor maps are not available") : s;
 }
 
 }  // extern "C"

@@ -48,15 +48,18 @@ constexpr int PA_KST = 3;
 // on to kc before its slot had been filled. With an even number of barriers each has one issuer, which sees all of its phases.
 constexpr int PA_KBAR = 2 * PA_KST;
 constexpr int PA_OFF_K = 0;                            // (the query tile lives in tensor memory, not here)
-// prefill_attn_kernel serves two shapes. MLA prefill (its exact form): 192-wide expanded keys, the 512 value columns in two halves, three
+// prefill_attn_kernel serves three shapes. MLA prefill (its exact form): 192-wide expanded keys, the 512 value columns in two halves, three
 // value stages. GQA prefill (Qwen3.5 layers): 256-wide keys and values of one KV head, two value stages (the key tiles are
-// 32 KB instead of 24 KB). Shared-memory layout and the query tile's width in tensor memory follow from DQK and CST.
-template <int DQK_, int CST_>
+// 32 KB instead of 24 KB); and 128-wide ones (the chunk over a cache held in 8 bits). Shared-memory layout and the query tile's width in
+// tensor memory follow from DQK, CST and the width DV of the accumulator.
+template <int DQK_, int CST_, int DV_ = PA_DV>
 struct PaCfg {
-    static constexpr int DQK = DQK_, CST = CST_;
+    static constexpr int DQK = DQK_, CST = CST_, DV = DV_;
+    static constexpr int C_BYTES = PA_KT * DV * 2;     // DV / 64 blocks of [64][64]
+    static constexpr int RECORD = PA_QT * (DV + 2);    // floats: O as [DV / 4][row][4], m [row], l [row]
     static constexpr int K_BYTES = PA_KT * DQK * 2;    // 24576 / 32768: DQK / 64 blocks of [64][64]
     static constexpr int OFF_C = PA_OFF_K + PA_KST * K_BYTES;
-    static constexpr int OFF_P = OFF_C + CST * PA_C_BYTES;
+    static constexpr int OFF_P = OFF_C + CST * C_BYTES;
     static constexpr int OFF_BAR = OFF_P + 2 * PA_P_BYTES;
     static constexpr int OFF_X = OFF_BAR + 512;        // [4][128] f32 maxima, [4][128] f32 sums exchanged between the softmax groups; 8 items of 16 bytes
     static constexpr int SMEM = OFF_X + 4096 + 128 + 1024;
@@ -65,6 +68,7 @@ struct PaCfg {
 };
 using PaMla = PaCfg<192, 3>;
 using PaGqa = PaCfg<256, 2>;
+using PaGqa128 = PaCfg<128, 3, 128>;
 static_assert(PaMla::OFF_BAR == 204800, "shared-memory budget");
 constexpr uint32_t PA_COL_O = 0, PA_COL_S = 256, PA_COL_Q = 384;   // S buffers at 256 and 320; Q: DQK / 2 columns of bf16 pairs
 constexpr float PA_LAZY = 8.f;                         // exact form: rescale when a score outruns the reference by 2^8
@@ -204,7 +208,7 @@ template <int NWG, class CFG, bool GQA>      // NWG softmax warp groups: 4 = fas
 __global__ void __launch_bounds__(PA_THREADS<NWG>, 1)
 prefill_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_c, const AttnParams p) {
     constexpr int PA_DQK = CFG::DQK, PA_K_BYTES = CFG::K_BYTES, PA_CST = CFG::CST, PA_OFF_C = CFG::OFF_C, PA_OFF_P = CFG::OFF_P,
-                  PA_OFF_BAR = CFG::OFF_BAR, PA_OFF_X = CFG::OFF_X;
+                  PA_OFF_BAR = CFG::OFF_BAR, PA_OFF_X = CFG::OFF_X, PA_DV = CFG::DV, PA_C_BYTES = CFG::C_BYTES;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -331,7 +335,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                     ok = mbar_wait(bar(PB_CEMPTY + cs), (uint32_t)((cu & 1) ^ 1), p.err, 1002);
                     if (!ok) break;
                     mbar_expect_tx(bar(PB_CFULL + cs), PA_C_BYTES);
-                    tma_load_3d(base + PA_OFF_C + cs * PA_C_BYTES, &tm_c, 0, i * PA_KT, (GQA ? it.h / p.group : it.half) * 4, bar(PB_CFULL + cs));
+                    tma_load_3d(base + PA_OFF_C + cs * PA_C_BYTES, &tm_c, 0, i * PA_KT, (GQA ? it.h / p.group : it.half) * (PA_DV / 64), bar(PB_CFULL + cs));
                 }
             }
             if (!ok)
@@ -578,7 +582,7 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
                 l = (s_l[row] + s_l[128 + row]) + (s_l[256 + row] + s_l[384 + row]);
             }
             if (it.rec >= 0) {                                       // part of an item: its record
-                float *rec = p.records + record_of<GQA>(it.rec, half) * PA_RECORD;
+                float *rec = p.records + record_of<GQA>(it.rec, half) * CFG::RECORD;
                 constexpr int CPG = PA_DV / NWG;                     // columns per group
 #pragma unroll 1
                 for (int c = 0; c < CPG / 16; c++) {
@@ -602,22 +606,20 @@ prefill_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
             // no other warp writes.
             uint8_t *stg = sm + PA_OFF_P + (warp - 4) * (NWG == 4 ? 2048 : 32 * 128);
             const int t0w = q0 + q4 * 32;
-            constexpr int NCH = PA_DV / 64 / NWG;                     // 64-column chunks per thread
+            constexpr int CW = PA_DV / NWG < 64 ? PA_DV / NWG : 64, NCH = PA_DV / CW / NWG;      // columns at a time; such chunks per thread
 #pragma unroll 1
             for (int c = 0; c < NCH; c++) {
-                const int col = (wg * NCH + c) * 64;
-                uint32_t o[64];
-                TMEM_LD16(o, 0, tlane + PA_COL_O + col);
-                TMEM_LD16(o, 16, tlane + PA_COL_O + col + 16);
-                TMEM_LD16(o, 32, tlane + PA_COL_O + col + 32);
-                TMEM_LD16(o, 48, tlane + PA_COL_O + col + 48);
+                const int col = (wg * NCH + c) * CW;
+                uint32_t o[CW];
+#pragma unroll
+                for (int u = 0; u < CW; u += 16) TMEM_LD16(o, u, tlane + PA_COL_O + col + u);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                 if (c == NCH - 1) {
                     tc_fence_before();
                     arrive(PB_OFREE);                                // the value MMAs of the next item may overwrite the accumulator
                 }
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
+                for (int u = 0; u < CW / 32; u++) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const uint32_t *x = o + u * 32 + 8 * j;
@@ -1126,8 +1128,9 @@ prefill_pair_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
 // queries after 10488 rows, 39 MB of records, 12.8 -> 8.9 us (sixteen columns and 64-bit divisions before; asking for the next
 // segment's columns before the addition of this one's: 10.4, in registers that blocks then lack).
 constexpr int PA_MC = 32;                                            // columns per thread
-template <bool GQA>
+template <class CFG, bool GQA>
 __global__ void __launch_bounds__(128) attn_merge_kernel(const AttnParams p) {
+    constexpr int PA_DV = CFG::DV;
     cwk_pdl_launch();
     const int nq = (p.n + PA_QT - 1) / PA_QT, row = threadIdx.x, c0 = (int)blockIdx.y * PA_MC, half = blockIdx.z;
     const int all = p.head_tiles * p.nh;
@@ -1151,7 +1154,7 @@ __global__ void __launch_bounds__(128) attn_merge_kernel(const AttnParams p) {
         for (; g <= g1; g++) {
             AttnItem seg = it;
             if (!attn_segment(seg, w, g, at, share_begin(g, all, p.shares), share_begin(g + 1, all, p.shares), p)) continue;
-            const float *rec = p.records + record_of<GQA>(seg.rec, half) * PA_RECORD;
+            const float *rec = p.records + record_of<GQA>(seg.rec, half) * CFG::RECORD;
 #pragma unroll
             for (int j = 0; j < PA_MC / 4; j++) v[j] = *reinterpret_cast<const float4 *>(rec + ((int64_t)(c0 / 4 + j) * PA_QT + row) * 4);
             ms = rec[PA_QT * PA_DV + row];
@@ -1214,7 +1217,7 @@ int attn_launch(cwk_ctx *ctx, AttnParams ap, const CUtensorMap &tm_k, const CUte
     const int64_t one_by_one = std::max(tiles(nq - 1), share + (waves * G - total) * tiles(0) / G);
     ap.shares = 0; ap.records = nullptr; ap.head_tiles = (int)head_tiles;
     if (one_by_one > share + (GQA ? (int64_t)PA_MERGE_TILES : std::max<int64_t>(PR_MERGE_TILES, share / 4)) && share >= 2 && all < (1LL << 31)) {
-        const int s = cwk_reserve_scratch(ctx, (size_t)2 * H * G * PA_RECORD * sizeof(float));
+        const int s = cwk_reserve_scratch(ctx, (size_t)2 * H * G * CFG::RECORD * sizeof(float));
         if (s != CWK_OK) return s;
         ap.shares = G; ap.records = ctx->scratch;
     }
@@ -1236,7 +1239,7 @@ int attn_launch(cwk_ctx *ctx, AttnParams ap, const CUtensorMap &tm_k, const CUte
     CWK_CUDA(ctx, cwk_launch_early(prefill_attn_kernel<1, CFG, GQA>, dim3(ap.shares ? H * G : std::min(H * total, ctx->sm_count)), dim3(PA_THREADS<1>), CFG::SMEM, ctx->stream, tm_k, tm_c, ap));
     CWK_LAUNCH_CHECK(ctx, "prefill_attn_kernel<1>");
     if (ap.shares) {
-        CWK_CUDA(ctx, cwk_launch_early(attn_merge_kernel<GQA>, dim3(ap.shares, PA_DV / PA_MC, H), dim3(128), 0, ctx->stream, ap));
+        CWK_CUDA(ctx, cwk_launch_early(attn_merge_kernel<CFG, GQA>, dim3(ap.shares, CFG::DV / PA_MC, H), dim3(128), 0, ctx->stream, ap));
         CWK_LAUNCH_CHECK(ctx, "attn_merge_kernel");
     }
     return CWK_OK;
@@ -1473,19 +1476,20 @@ int cwk_mla_prefill_attn_tc(cwk_ctx *ctx, const void *Q, const float *rot, const
 // tensor path cannot take the operands.
 int cwk_gqa_prefill_tc(cwk_ctx *ctx, const void *Q, const void *K, const void *V, int64_t pos, int n, int nh, int nkv, int hd,
                        float scale, void *out, int *flags) {
-    if (!cwk_encode_tiled_fn() || hd != 256 || nkv <= 0 || nh % nkv) return CWK_ERR_UNSUPPORTED;
+    if (!cwk_encode_tiled_fn() || (hd != 256 && hd != 128) || nkv <= 0 || nh % nkv) return CWK_ERR_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V) | reinterpret_cast<uintptr_t>(out)) & 15)
         return CWK_ERR_UNSUPPORTED;
     int s = cwk_ensure_err_word(ctx);
     if (s != CWK_OK) return s;
     const int T = (int)(pos + n);
     CUtensorMap tm_k, tm_v;
-    // the caches as [64][rows][nkv * 4 column blocks]: a tile is one box of 64 keys x the 4 blocks of one KV head
-    if (!encode3(&tm_k, K, (uint64_t)T, (uint64_t)nkv * 4, (uint64_t)nkv * hd * 2, PA_KT, 4) ||
-        !encode3(&tm_v, V, (uint64_t)T, (uint64_t)nkv * 4, (uint64_t)nkv * hd * 2, PA_KT, 4))
+    // the caches as [64][rows][nkv * hd / 64 column blocks]: a tile is one box of 64 keys x the blocks of one KV head
+    const int blocks = hd / 64;
+    if (!encode3(&tm_k, K, (uint64_t)T, (uint64_t)nkv * blocks, (uint64_t)nkv * hd * 2, PA_KT, blocks) ||
+        !encode3(&tm_v, V, (uint64_t)T, (uint64_t)nkv * blocks, (uint64_t)nkv * hd * 2, PA_KT, blocks))
         return cwk_fail(ctx, CWK_ERR_CUDA, "cuTensorMapEncodeTiled failed for the GQA prefill operands");
     AttnParams ap{};
     ap.q = (const uint16_t *)Q; ap.out = (uint16_t *)out; ap.n = n; ap.nh = nh; ap.T = T; ap.pos0 = pos; ap.group = nh / nkv;
     ap.scale_log2 = scale * 1.4426950408889634f; ap.flags = flags; ap.err = ctx->dev_err;
-    return attn_launch<PaGqa, true>(ctx, ap, tm_k, tm_v, 0);
+    return hd == 256 ? attn_launch<PaGqa, true>(ctx, ap, tm_k, tm_v, 0) : attn_launch<PaGqa128, true>(ctx, ap, tm_k, tm_v, 0);
 }

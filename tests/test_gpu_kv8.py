@@ -318,7 +318,8 @@ def test_decode_gives_the_same_bits_again(attn):
 
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])
 @pytest.mark.parametrize("n,pos,nh,nkv,hd", [(1, 0, 4, 1, 256), (1, 700, 16, 4, 256), (3, 500, 16, 4, 128), (17, 300, 8, 8, 256), (64, 0, 16, 1, 256),
-                                             (200, 37, 16, 4, 256), (129, 0, 16, 4, 128), (257, 1300, 8, 2, 256), (300, 1, 4, 4, 128)])
+                                             (200, 37, 16, 4, 256), (129, 0, 16, 4, 128), (257, 1300, 8, 2, 256), (300, 1, 4, 4, 128),
+                                             (700, 0, 24, 3, 128), (150, 3000, 16, 2, 128), (520, 2800, 6, 2, 128), (130, 700, 20, 1, 256), (5, 70, 20, 1, 128)])
 def test_prefill_against_64_bits(attn, kind, n, pos, nh, nkv, hd):
     T = pos + n
     rows = -(-T // 64) * 64
@@ -443,6 +444,6 @@ def test_refusals(attn):
            L.cwk_gqa_prefill_kv8(h, p(q), a, 0, -1, 2, 8, 1.0, p(o)), L.cwk_gqa_prefill_kv8(h, p(q), a, -1, 0, 2, 8, 1.0, p(o))]
     assert bad == [cl.ERR_ARGUMENT] * len(bad)
     bad = [L.cwk_gqa_qk_prep_kv8(h, p(f), p(f), p(f), p(f), p(f), 1e-6, 24, 1e4, p(pos), None, 2, 1, 8, p(o), a),
-           L.cwk_gqa_decode_kv8(h, p(q), a, p(pos), 64, 2, 1, 34, 1.0, p(o), 0), L.cwk_gqa_prefill_kv8(h, p(q), a, 0, 0, 2, 34, 1.0, p(o))]
+           L.cwk_gqa_decode_kv8(h, p(q), a, p(pos), 64, 2, 1, 34, 1.0, p(o), 0)]
     assert bad == [cl.ERR_UNSUPPORTED] * len(bad)
     attn.ctx.sync()
