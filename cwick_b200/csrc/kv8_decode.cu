@@ -432,25 +432,68 @@ int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *o
 
 }  // namespace
 
+namespace {
+
+// The shape of a pass of the streams over `B` sequences of up to `len` rows.
+struct Kv8Shape {
+    int hb, per, parts, keys, blocks;
+    int64_t groups, steps;            // steps: at most
+    Kv8Shape(int sm_count, int B, int64_t len, int n, int nh, int nkv, int max_blocks) {
+        const int group = nh / nkv;
+        hb = nkv % 4 == 0 ? 4 : nkv % 2 == 0 ? 2 : 1;
+        per = std::min(n, std::max(1, 16 / group));
+        parts = (n + per - 1) / per;
+        keys = GK * (GW / hb);
+        groups = (int64_t)(nkv / hb) * parts;
+        steps = B * groups * ((len + keys - 1) / keys);
+        // as many blocks as there can be steps, at most two per SM
+        blocks = (int)std::min<int64_t>(std::max<int64_t>(1, steps), max_blocks > 0 ? std::min(max_blocks, 2 * sm_count) : 2 * sm_count);
+    }
+    int cols(int group) const { return per * group; }
+};
+
+// Which way a chunk goes. The streams read the codes once for every 16 query rows, every row over all keys; the tensor-core kernel has 128
+// query tokens of a head in a tile, but wants the cache widened and three or four launches. Fitted to 580 chunks of 4 to 300 tokens after 0 to 12000
+// rows, (16, 4), (8, 1), (8, 8), (32, 2), (24, 3) and (16, 2) heads, us a call replayed (mean error 5 to 12 %; the choice costs 1.5 % of the better
+// side's time on average). Streams / tensor cores, 16 heads, 4 KV heads of 256: 4 tokens after 2000 rows 11 / 37, 37 after 2500 28 / 38, 128 after 2000
+// 53 / 41, 64 after 12000 81 / 65; of 128: 64 after 2000 19 / 30, 200 after 12000 122 / 55.
+bool kv8_streams_sooner(int sm_count, int64_t pos, int n, int nh, int nkv, int hd) {
+    const int group = nh / nkv;
+    if (group > 16) return false;
+    const int64_t T = pos + n;
+    const bool wide = hd == 256;
+    const Kv8Shape s(sm_count, 1, T, n, nh, nkv, 0);
+    const double turns = (double)((s.steps + s.blocks - 1) / s.blocks), records = (double)s.blocks * GW * s.cols(group) * hd * 4e-6;
+    const double streams = (wide ? 6.8 : 6.0) + turns * (s.cols(group) <= 8 ? (wide ? 0.94 : 0.82) : (wide ? 3.1 : 1.85)) + 0.65 * records;
+    // items of 128 tokens x one head, 64 keys a tile; where the longest block has many tiles above an equal share they are dealt out in shares and joined
+    const int64_t items = (int64_t)((n + 127) / 128) * nh;
+    const auto tiles = [&](int64_t last) { return (last + 63) / 64; };
+    int64_t all = 0;
+    for (int64_t q = 0; q < n; q += 128) all += tiles(pos + std::min<int64_t>(q + 128, n)) * nh;
+    const int64_t share = (all + sm_count - 1) / sm_count, idle = ((items + sm_count - 1) / sm_count) * sm_count - items;
+    const int64_t dealt = std::max(tiles(T), share + idle * tiles(pos + std::min(128, n)) / sm_count);
+    const bool shared = dealt > share + 28;
+    const double tensor = (wide ? 15.5 : 14.3) + (double)(shared ? share : dealt) * (wide ? 0.64 : 0.54) + (shared ? (wide ? 17.4 : 14.0) : 0.0) + (double)T * nkv * hd * 6 * 0.256e-6;
+    return streams < tensor;
+}
+
+}  // namespace
+
 int cwk_kv8_streams(cwk_ctx *ctx, const void *q, const cwk_kv8 &c, const int32_t *kv_len, int max_kv_len, int B, int n, int nh, float scale,
                     void *out, int max_blocks) {
     Kv8DecodeParams p{};
     p.q = (const uint16_t *)q; p.k = (const uint8_t *)c.k; p.v = (const uint8_t *)c.v; p.ks = c.k_scale; p.vs = c.v_scale; p.rows = c.rows;
-    p.n = n; p.nh = nh; p.nkv = c.nkv; p.group = nh / c.nkv; p.hb = c.nkv % 4 == 0 ? 4 : c.nkv % 2 == 0 ? 2 : 1;
+    const Kv8Shape shape(ctx->sm_count, B, max_kv_len, n, nh, c.nkv, max_blocks);
+    const int blocks = shape.blocks;
+    p.n = n; p.nh = nh; p.nkv = c.nkv; p.group = nh / c.nkv; p.hb = shape.hb; p.per = shape.per; p.parts = shape.parts;
     p.lb = c.block == 32 ? 5 : c.block == 64 ? 6 : 7;
-    p.per = std::min(n, std::max(1, 16 / p.group));
-    p.parts = (n + p.per - 1) / p.per;
     p.scale_log2 = scale * 1.4426950408889634f;
-    // as many blocks as there can be steps, at most two per SM
-    const int keys = GK * (GW / p.hb);
-    const int64_t groups = (int64_t)(c.nkv / p.hb) * p.parts;
-    const int64_t most = std::max<int64_t>(1, B * groups * ((max_kv_len + keys - 1) / keys));
-    const int blocks = (int)std::min<int64_t>(most, max_blocks > 0 ? std::min(max_blocks, 2 * ctx->sm_count) : 2 * ctx->sm_count);
-    const size_t rec_bytes = (size_t)(B * groups + blocks) * GW * kv8_record(p.per * p.group, c.hd) * sizeof(float);
-    const int s = cwk_reserve_scratch(ctx, rec_bytes + (size_t)B * groups * sizeof(int2));
+    if (shape.groups > 0x7FFFFFFF) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_decode_kv8: too many query tokens");
+    const size_t rec_bytes = (size_t)(B * shape.groups + blocks) * GW * kv8_record(shape.cols(p.group), c.hd) * sizeof(float);
+    const int s = cwk_reserve_scratch(ctx, rec_bytes + (size_t)B * shape.groups * sizeof(int2));
     if (s != CWK_OK) return s;
     p.rec = ctx->scratch;
-    p.steps = GqaSteps{kv_len, B, (int)groups, keys, kv_len ? (int)c.rows : max_kv_len, (int2 *)((uint8_t *)ctx->scratch + rec_bytes)};
+    p.steps = GqaSteps{kv_len, B, (int)shape.groups, shape.keys, kv_len ? (int)c.rows : max_kv_len, (int2 *)((uint8_t *)ctx->scratch + rec_bytes)};
     if (p.per * p.group > 8) return c.hd == 256 ? launch<256, 2>(ctx, p, c.type, blocks, out) : launch<128, 2>(ctx, p, c.type, blocks, out);
     return c.hd == 256 ? launch<256, 1>(ctx, p, c.type, blocks, out) : launch<128, 1>(ctx, p, c.type, blocks, out);
 }
@@ -483,11 +526,12 @@ int cwk_gqa_prefill_kv8(cwk_ctx *ctx, const void *Q, const cwk_kv8 *c, int slot,
         return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_prefill_kv8: bad dimensions");
     if ((((uintptr_t)Q | (uintptr_t)out) & 15) != 0) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_prefill_kv8: pointers must be 16-byte aligned");
     CWK_CUDA(ctx, cudaSetDevice(ctx->device));
-    // the slot's rows widened, exactly, behind the flags that the bf16 kernel keeps at the start of the workspace (a word per item and SM)
     cwk_kv8 at = *c;
     const int64_t T = pos + n, row = (int64_t)c->nkv * c->hd;
     at.k = (uint8_t *)c->k + slot * c->rows * row; at.v = (uint8_t *)c->v + slot * c->rows * row;
     at.k_scale = c->k_scale + slot * (c->rows / c->block) * c->nkv; at.v_scale = c->v_scale + slot * (c->rows / c->block) * c->nkv;
+    if (kv8_streams_sooner(ctx->sm_count, pos, n, nh, c->nkv, c->hd)) return cwk_kv8_streams(ctx, Q, at, nullptr, (int)T, 1, n, nh, scale, out, 0);
+    // the slot's rows widened, exactly, behind the flags that the bf16 kernel keeps at the start of the workspace (a word per item and SM)
     const size_t flags = ((((size_t)((n + 127) / 128) * nh + ctx->sm_count + 3) * sizeof(int)) + 255) & ~(size_t)255, half = (size_t)T * row * 2;
     s = cwk_reserve_work(ctx, flags + 2 * half);
     if (s != CWK_OK) return s;
