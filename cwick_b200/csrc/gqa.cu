@@ -43,7 +43,7 @@ static int gqa_prefill_launch(cwk_ctx *ctx, const FlashRowsParams &p, int nblock
 int cwk_gqa_decode_streams(cwk_ctx *ctx, const void *q, const void *K, const void *V, int64_t seq_stride, const int32_t *kv_len, int max_kv_len,
                            const int32_t *sel, int64_t sel_ld, int B, int nh, int nkv, int hd, float scale, void *out, int max_blocks);
 int cwk_gqa_prefill_tc(cwk_ctx *ctx, const void *Q, const void *K, const void *V, int64_t pos, int n, int nh, int nkv, int hd,
-                       float scale, void *out, int *flags);
+                       float scale, void *out, int *flags, int spread);
 
 extern "C" {
 
@@ -134,7 +134,7 @@ int cwk_gqa_prefill(cwk_ctx *ctx, const void *Q, const void *K, const void *V, i
         const size_t flags_bytes = ((size_t)((n + 127) / 128) * nh + ctx->sm_count + 3) * sizeof(int);
         int s = cwk_reserve_work(ctx, flags_bytes);
         if (s != CWK_OK) return s;
-        s = cwk_gqa_prefill_tc(ctx, Q, K, V, pos, n, nh, nkv, hd, scale, out, (int *)ctx->work);
+        s = cwk_gqa_prefill_tc(ctx, Q, K, V, pos, n, nh, nkv, hd, scale, out, (int *)ctx->work, 0);
         if (s != CWK_ERR_UNSUPPORTED) return s;
     }
     const int QT = 64 / group;

@@ -500,7 +500,7 @@ int cwk_kv8_streams(cwk_ctx *ctx, const void *q, const cwk_kv8 &c, const int32_t
 
 // mla_prefill_attn.cu
 int cwk_gqa_prefill_tc(cwk_ctx *ctx, const void *Q, const void *K, const void *V, int64_t pos, int n, int nh, int nkv, int hd,
-                       float scale, void *out, int *flags);
+                       float scale, void *out, int *flags, int spread);
 
 extern "C" {
 
@@ -538,7 +538,7 @@ int cwk_gqa_prefill_kv8(cwk_ctx *ctx, const void *Q, const cwk_kv8 *c, int slot,
     uint8_t *wk = (uint8_t *)ctx->work + flags;
     s = cwk_kv8_widen(ctx, at, 0, T, wk, wk + half);
     if (s != CWK_OK) return s;
-    s = cwk_gqa_prefill_tc(ctx, Q, wk, wk + half, pos, n, nh, c->nkv, c->hd, scale, out, (int *)ctx->work);
+    s = cwk_gqa_prefill_tc(ctx, Q, wk, wk + half, pos, n, nh, c->nkv, c->hd, scale, out, (int *)ctx->work, 2 * half <= (size_t)64 << 20);
     return s == CWK_ERR_UNSUPPORTED ? cwk_fail(ctx, s, "gqa_prefill_kv8: tensor maps are not available") : s;
 }
 

@@ -87,6 +87,7 @@ struct AttnParams {
     int group;          // GQA: query heads per KV head (MLA: unused)
     int64_t pos0;
     float scale_log2;
+    int spread;         // items of all heads from the longest to the shortest
     int *flags;         // one word per item (share mode: per item + share): fast form sets it, exact form runs only where it is set
     int *counter;       // [3]: item counters of the fast and the exact form, number of flags raised; zero at launch
     int *err;
@@ -105,12 +106,13 @@ struct AttnItem {
 };
 
 // Work item w of the attention grid: query tiles from the longest to the shortest inside one head, then the next head: blocks that
-// run at the same time work on the same few heads, whose keys stay in L2. (MLA: each of the two halves of the value columns does it.)
+// run at the same time work on the same few heads, whose keys stay in L2. (spread: the longest of all heads first, for keys that all stay there:
+// a head whose longest items begin last is waited for, 2000 tokens of 24 heads of 128 58.7 us against 51.6.) (MLA: each of the two halves of the value columns does it.)
 __device__ __forceinline__ AttnItem attn_item(int w, const AttnParams &p, int nq) {
     AttnItem it;
-    const int qtile = nq - 1 - (w % nq);
+    const int qtile = nq - 1 - (p.spread ? w / p.nh : w % nq);
     it.q0 = qtile * PA_QT;
-    it.h = w / nq;
+    it.h = p.spread ? w % p.nh : w / nq;
     it.half = 0;
     const int64_t last_q = p.pos0 + min(it.q0 + PA_QT - 1, p.n - 1);     // keys 0 .. pos0 + (last query of the item): tiles of 64
     it.lo = 0;
@@ -1219,7 +1221,7 @@ int attn_launch(cwk_ctx *ctx, AttnParams ap, const CUtensorMap &tm_k, const CUte
     if (one_by_one > share + (GQA ? (int64_t)PA_MERGE_TILES : std::max<int64_t>(PR_MERGE_TILES, share / 4)) && share >= 2 && all < (1LL << 31)) {
         const int s = cwk_reserve_scratch(ctx, (size_t)2 * H * G * CFG::RECORD * sizeof(float));
         if (s != CWK_OK) return s;
-        ap.shares = G; ap.records = ctx->scratch;
+        ap.shares = G; ap.records = ctx->scratch; ap.spread = 0;
     }
     const int nflags = total + (ap.shares ? G : 0);
     ap.counter = ap.flags + nflags;
@@ -1475,7 +1477,7 @@ int cwk_mla_prefill_attn_tc(cwk_ctx *ctx, const void *Q, const float *rot, const
 // [n][nh][256]; flags = workspace int32 [ceil(n / 128) * nh + number of SMs + 3]. Returns CWK_ERR_UNSUPPORTED (no error text) when the
 // tensor path cannot take the operands.
 int cwk_gqa_prefill_tc(cwk_ctx *ctx, const void *Q, const void *K, const void *V, int64_t pos, int n, int nh, int nkv, int hd,
-                       float scale, void *out, int *flags) {
+                       float scale, void *out, int *flags, int spread) {
     if (!cwk_encode_tiled_fn() || (hd != 256 && hd != 128) || nkv <= 0 || nh % nkv) return CWK_ERR_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(Q) | reinterpret_cast<uintptr_t>(K) | reinterpret_cast<uintptr_t>(V) | reinterpret_cast<uintptr_t>(out)) & 15)
         return CWK_ERR_UNSUPPORTED;
@@ -1490,6 +1492,6 @@ int cwk_gqa_prefill_tc(cwk_ctx *ctx, const void *Q, const void *K, const void *V
         return cwk_fail(ctx, CWK_ERR_CUDA, "cuTensorMapEncodeTiled failed for the GQA prefill operands");
     AttnParams ap{};
     ap.q = (const uint16_t *)Q; ap.out = (uint16_t *)out; ap.n = n; ap.nh = nh; ap.T = T; ap.pos0 = pos; ap.group = nh / nkv;
-    ap.scale_log2 = scale * 1.4426950408889634f; ap.flags = flags; ap.err = ctx->dev_err;
+    ap.scale_log2 = scale * 1.4426950408889634f; ap.flags = flags; ap.err = ctx->dev_err; ap.spread = spread;
     return hd == 256 ? attn_launch<PaGqa, true>(ctx, ap, tm_k, tm_v, 0) : attn_launch<PaGqa128, true>(ctx, ap, tm_k, tm_v, 0);
 }
