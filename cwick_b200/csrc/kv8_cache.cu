@@ -29,7 +29,7 @@ struct Kv8WriteParams {
     int heads;                                 // query heads per warp
     double freq_hi[16], freq_lo[8];            // angle per position of pair i: freq_hi[i / 8] * freq_lo[i % 8]
 };
-constexpr int KQ_HEADS = 4;                    // most query heads of a warp
+constexpr int KQ_HEADS = 8;                    // most query heads of a warp
 
 // new rows of slot b: positions pos .. pos + the result - 1, all inside the slot
 __device__ __forceinline__ int new_rows(const Kv8WriteParams &p, int b, int64_t &pos) {
@@ -451,7 +451,7 @@ struct Kv8ReadParams {
     int64_t n;
     void *k, *v;
 };
-constexpr int KR_THREADS = 256, KR_ROWS = 8;
+constexpr int KR_THREADS = 128, KR_ROWS = 4;
 
 // A thread has eight codes (head, place in it) of every `step`-th row of a slot, KR_ROWS rows in flight. grid (chunks of rows, slot, K or V)
 template <int HD, bool I8, bool F32>
@@ -531,7 +531,7 @@ int launch_write_rows(cwk_ctx *ctx, Kv8WriteParams &p, int type) {
     size_t smem = 0;
     auto kern = type == CWK_KV8_INT8 ? kv8_write_kernel<V, SRC, true, PREP, ROWS> : kv8_write_kernel<V, SRC, false, PREP, ROWS>;
     if (PREP) {
-        p.heads = p.n * (int64_t)p.B * p.nh <= 16 * 1024 ? 1 : KQ_HEADS;      // query heads that share a token's angles; few rows: one warp each
+        p.heads = p.n * (int64_t)p.B * p.nh <= 2048 ? 1 : KQ_HEADS;      // query heads that share a token's angles and are on their way together; few rows: a warp each
         blocks += ((int64_t)p.B * p.n * ((p.nh + p.heads - 1) / p.heads) + warps - 1) / warps;
         smem = (size_t)(p.rot / 2) * warps * ROWS * sizeof(float2);      // 128 KB at most (32 KB for 64 values in blocks of 128 rows)
         static bool attr_set[2][16] = {};
