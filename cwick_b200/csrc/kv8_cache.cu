@@ -72,15 +72,16 @@ __device__ __forceinline__ uint32_t finite_magnitude(float x) {
 }
 
 // float -> double in integer work: the conversion instructions of 64-bit types run at a small part of the rate of the arithmetic (with
-// them the keys of 2100 tokens took 38 us, most of the time in conversions). Subnormals are zero.
+// them the keys of 2100 tokens took 38 us, most of the time in conversions). Not for subnormals.
 __device__ __forceinline__ double wide(float x) {
-    const uint32_t u = __float_as_uint(x), e = u & 0x7F800000u, sign = u & 0x80000000u;
-    const uint32_t hi = sign | (((u & 0x7FFFFFFFu) >> 3) + 0x38000000u) | (e == 0x7F800000u ? 0x7FF00000u : 0u);
-    return __hiloint2double((int)(e ? hi : sign), (int)(e ? u << 29 : 0u));
+    const uint32_t u = __float_as_uint(x), e = u & 0x7F800000u;
+    const uint32_t hi = (u & 0x80000000u) | (((u & 0x7FFFFFFFu) >> 3) + 0x38000000u) | (e == 0x7F800000u ? 0x7FF00000u : 0u);
+    return __hiloint2double((int)(e ? hi : u), (int)(e ? u << 29 : 0u));
 }
-template <class T> __device__ __forceinline__ T as(float x);
-template <> __device__ __forceinline__ float as<float>(float x) { return x; }
-template <> __device__ __forceinline__ double as<double>(float x) { return wide(x); }
+__device__ __forceinline__ bool subnormal(float x) {
+    const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
+    return u - 1u < 0x7FFFFFu;
+}
 
 // The angle of pair i per position.
 __device__ __forceinline__ double frequency(const Kv8WriteParams &p, int i) { return p.freq_hi[i >> 3] * p.freq_lo[i & 7]; }
@@ -127,7 +128,7 @@ __device__ __forceinline__ int partner(int rot, int lane) {
 template <int V, class T, class X, class CS>
 __device__ __forceinline__ void norm_rotate(const X &x, T rstd, const T (&w1)[V], int rot, int lane, const CS *cs, T (&y)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; i++) y[i] = as<T>(x[i]) * rstd * w1[i];
+    for (int i = 0; i < V; i++) y[i] = x[i] * rstd * w1[i];
     if (rot == 0) return;
     const int d0 = lane * V, from = partner<V>(rot, lane), pair = d0 < rot / 2 ? d0 : d0 - rot / 2;
     const bool lo = d0 < rot / 2, hi = !lo && d0 < rot;
@@ -146,7 +147,7 @@ __device__ __forceinline__ T squares(const X &x) {
     T sum = 0;
 #pragma unroll
     for (int i = 0; i < V; i += 4) {
-        const T a = as<T>(x[i]), b = as<T>(x[i + 1]), c = as<T>(x[i + 2]), d = as<T>(x[i + 3]);
+        const T a = x[i], b = x[i + 1], c = x[i + 2], d = x[i + 3];
         sum += (a * a + b * b) + (c * c + d * d);
     }
     return sum;
@@ -329,11 +330,19 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
         auto row64 = [&](int r, double (&y)[V]) {
             Raw<V, SRC> z;
             z.load(src, row + r * p.nkv, lane);
-            double w1[V];
+            double x64[V], w1[V];
+            bool some = false;
 #pragma unroll
-            for (int i = 0; i < V; i++) w1[i] = 1.0 + wide(w[i]);
+            for (int i = 0; i < V; i++) {
+                x64[i] = wide(z[i]);
+                w1[i] = 1.0 + wide(w[i]);
+                some |= subnormal(z[i]);
+            }
+            if (some)                                      // (an ordinary row has none)
+#pragma unroll
+                for (int i = 0; i < V; i++) x64[i] = (double)z[i];
             angles(p, pairs, lo + first + r, lane, cs);
-            norm_rotate<V, double>(z, rsqrt(warp_sum(squares<V, double>(z)) / (double)HD + (double)p.eps), w1, p.rot, lane, cs, y);
+            norm_rotate<V, double>(x64, rsqrt(warp_sum(squares<V, double>(x64)) / (double)HD + (double)p.eps), w1, p.rot, lane, cs, y);
         };
         float y[ROWS][V];
         uint32_t amax = 0;

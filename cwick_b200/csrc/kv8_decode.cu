@@ -425,7 +425,7 @@ int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *o
     // Records per query row; the threads that a group of 16 for every 64 columns of a row makes. Groups as long as there are records for them
     // and the SMs are not filled more than once (37 tokens of 32 heads after 300 rows, 222 blocks, 12 records a row, 1184 rows: 26.8 us with eight
     // groups a row, 15.2 with one).
-    const int64_t each = (int64_t)blocks * (GW / p.hb) / ((int64_t)p.steps.B * p.parts), rows = p.n * p.nh, threads = rows * p.steps.B * (HD / 4);
+    const int64_t each = (int64_t)blocks * (GW / p.hb) / ((int64_t)p.steps.B * p.steps.groups), rows = p.n * p.nh, threads = rows * p.steps.B * (HD / 4);
     const int64_t room = std::min<int64_t>((int64_t)ctx->sm_count * 1536 / threads, each / 2);
     if (each > 8 && room >= 4) {
         const int groups = room >= 16 ? 16 : room >= 8 ? 8 : 4;

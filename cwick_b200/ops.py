@@ -43,6 +43,7 @@ class Kv8Cache:
         self.slots, self.rows, self.nkv, self.hd = slots, rows, nkv, hd
         self.c = _lib.Kv8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), rows, slots, nkv, hd, block, self.TYPES[type])
         self.address = _lib.C.addressof(self.c)
+        self.device = k.device.index
 
     @classmethod
     def empty(cls, slots, rows, nkv, hd, block=64, type="e4m3", device="cuda"):
@@ -207,7 +208,7 @@ class Attn:
     def kv8_store(self, cache, k, v, pos, count=None):
         """Rows pos[b] .. of slot b from k, v [B][n][nkv][hd] (bf16 or f32); pos, count int32 [B] cuda (count None: n rows each)."""
         B, n = k.shape[:2]
-        assert k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.is_contiguous() and v.is_contiguous()
+        assert cache.device == self.device and k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.is_contiguous() and v.is_contiguous()
         assert k.shape == v.shape == (B, n, cache.nkv, cache.hd)
         st = self._kv8_store(self.ctx.address, cache.address, k.data_ptr(), v.data_ptr(), 1 if k.dtype == torch.float32 else 0,
                              _i32(pos, B), _i32(count, B), B, n)
@@ -220,7 +221,7 @@ class Attn:
         if out is None:
             out = tuple(torch.empty(B, n, cache.nkv, cache.hd, dtype=dtype, device=cache.k.device) for _ in range(2))
         k, v = out
-        assert k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.is_contiguous() and v.is_contiguous()
+        assert cache.device == self.device and k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.is_contiguous() and v.is_contiguous()
         assert k.shape == v.shape == (B, n, cache.nkv, cache.hd)
         st = self._kv8_load(self.ctx.address, cache.address, _i32(pos, B), _i32(count, B), B, n, k.data_ptr(), v.data_ptr(),
                             1 if k.dtype == torch.float32 else 0)
@@ -234,7 +235,7 @@ class Attn:
         B, n, nh, _ = qg.shape
         for t in (qg, k, v, q_norm, k_norm):
             assert t.dtype == torch.float32 and t.is_contiguous()
-        assert qg.shape[3] == 2 * cache.hd and k.shape == v.shape == (B, n, cache.nkv, cache.hd) and q_norm.numel() == k_norm.numel() == cache.hd
+        assert cache.device == self.device and qg.shape[3] == 2 * cache.hd and k.shape == v.shape == (B, n, cache.nkv, cache.hd) and q_norm.numel() == k_norm.numel() == cache.hd
         if q_out is None:
             q_out = torch.empty(B, n, nh, cache.hd, dtype=torch.bfloat16, device=qg.device)
         assert _bf16(q_out).shape == (B, n, nh, cache.hd)
@@ -248,7 +249,7 @@ class Attn:
         """q bf16 [B][nh][hd], or [B][n][nh][hd] for n query tokens per sequence; kv_len int32 [B], those tokens' rows included."""
         _bf16(q)
         B, n, nh, hd = q.shape if q.dim() == 4 else (q.shape[0], 1, *q.shape[1:])
-        assert hd == cache.hd
+        assert hd == cache.hd and cache.device == self.device
         if scale is None:
             scale = 1.0 / math.sqrt(hd)
         if max_kv_len is None:
@@ -265,7 +266,7 @@ class Attn:
         """Q bf16 [n][nh][hd] at positions pos .. of a slot, whose rows up to pos + n are in the cache."""
         _bf16(Q)
         n, nh, hd = Q.shape
-        assert hd == cache.hd
+        assert hd == cache.hd and cache.device == self.device
         out = torch.empty_like(Q)
         self.ctx.check(self.lib.cwk_gqa_prefill_kv8(self.ctx.h, _p(Q), cache.address, slot, pos, n, nh, 1.0 / math.sqrt(hd) if scale is None else scale,
                                                     _p(out)))

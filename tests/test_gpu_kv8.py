@@ -209,6 +209,31 @@ def test_prep_against_64_bits(attn, kind, n, pos, count, nh, nkv, hd, rot, block
             assert np.array_equal(t[b, first:last].cpu().numpy(), w.codes[0])
 
 
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_prep_of_extreme_rows(attn, kind, eps):
+    """Rows whose squares leave float's range at either end, zero rows, infinities and NaN, next to ordinary ones: the float pass cannot
+    be trusted there, and codes and scales are still the definition's."""
+    nh, nkv, hd, rot, block, theta, n = 2, 2, 256, 64, 32, 1e4, 96
+    g = gen(5)
+    k, v = (torch.randn(1, n, nkv, hd, device="cuda", generator=g) for _ in range(2))
+    size = torch.ones(n, device="cuda")
+    size[3], size[4], size[40], size[41], size[42] = 1e30, 1e-30, 3e37, 1e-42, 0.0
+    k *= size[None, :, None, None]
+    v *= size[None, :, None, None]
+    k[0, 70, 0, 9], k[0, 71, 1, 200], v[0, 72, 0, 3], v[0, 73, 1, 4] = float("inf"), float("nan"), float("-inf"), float("nan")
+    qn, kn = (0.1 * torch.randn(hd, device="cuda", generator=g) for _ in range(2))
+    kn[100] = 1e6                                     # one channel far above the rest
+    c = cache_of(1, 128, nkv, hd, block, kind)
+    want = plain_of(c)
+    qg = torch.randn(1, n, nh, 2 * hd, device="cuda", generator=g)
+    attn.gqa_qk_prep_kv8(c, qg, k, v, qn, kn, eps, rot, theta, i32([7]))
+    with np.errstate(all="ignore"):
+        want[0].store(plain.norm_rotate(k[0].double().cpu().numpy(), kn.cpu().numpy(), eps, rot, theta, 7 + np.arange(n))[None], [7], [n])
+        want[1].store(v.double().cpu().numpy(), [7], [n])
+    same(c, want)
+
+
 # ---- decode -------------------------------------------------------------------------------------------------------------------
 
 def filled(attn, slots, rows, nkv, hd, block, kind, seed, climb=False):

@@ -44,6 +44,17 @@ def test_refusals_without_a_device(change, want):
     assert set(calls(L, None)) == {lib.ERR_ARGUMENT}
 
 
+@pytest.mark.parametrize("name", ["cwk_kv8_store", "cwk_kv8_load", "cwk_gqa_qk_prep_kv8", "cwk_gqa_decode_kv8"])
+def test_a_decode_steps_calls_are_in_the_compiled_binding(name):
+    L = lib.load()
+    fn = lib.fast(L, name)
+    assert type(fn).__name__ == "builtin_function_or_method"
+    args = [0.0 if a in (C.c_float, C.c_double) else None if a is C.c_void_p else 1 for a in lib.SIGNATURES[name][1]]
+    assert fn(*args) == lib.ERR_ARGUMENT == getattr(L, name)(*args)
+    with pytest.raises(TypeError):
+        fn(*args[:-1])
+
+
 def test_the_plain_codec_is_torchs():
     x = torch.cat([torch.randn(20000) * 60, torch.linspace(-2 ** -5, 2 ** -5, 4001), torch.tensor([448.0, 464.0, -1e30, 0.0, -0.0, 2.0 ** -10, 1.5 * 2.0 ** -9])])
     want = x.clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
