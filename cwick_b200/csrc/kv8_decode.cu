@@ -31,6 +31,7 @@ struct Kv8DecodeParams {
     int n, nh, nkv, group, hb, lb;    // hb: KV heads a block works on at once (4, 2 or 1); block = 1 << lb
     int per, parts;                   // query tokens whose heads share the MMA columns; parts = ceil(n / per)
     float scale_log2;
+    uint16_t *out;                    // bf16 [B][n][nh][hd]
     float *rec;                       // [slot][warp]: o [per * group][hd], then {m, l} [per * group]
     GqaSteps steps;                   // groups: (nkv / hb) * parts, the parts of the same keys next to each other; keys: GK * (GW / hb)
 };
@@ -61,8 +62,27 @@ __host__ __device__ __forceinline__ constexpr int kv8_record(int cols, int hd) {
 template <int HD, int NB> constexpr bool KV8_Q_SHARED = HD == 256 && NB == 2;
 template <int HD, int NB> constexpr int KV8_RING = KV8_Q_SHARED<HD, NB> ? 2 : HD == 256 ? 3 : 6;
 
-// NB: groups of eight MMA columns (query rows)
-template <int HD, int NB, bool I8>
+// A running softmax sum of one query row, four columns of it.
+struct Kv8Sum {
+    float M = -INFINITY, den = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    __device__ __forceinline__ void add(float w, float l, const float4 &v) {
+        den += w * l; o.x += w * v.x; o.y += w * v.y; o.z += w * v.z; o.w += w * v.w;
+    }
+    __device__ __forceinline__ void raise(float to) {      // to a reference exponent that is not lower
+        const float a = exp2f(M - to);
+        den *= a; o.x *= a; o.y *= a; o.z *= a; o.w *= a;
+        M = to;
+    }
+    __device__ __forceinline__ void write(uint16_t *out) const {
+        const float inv = den != 0.f ? 1.f / den : 0.f;
+        *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    }
+};
+
+// NB: groups of eight MMA columns (query rows). WHOLE: a block has one head group of one sequence from its first row to its last, joins its
+// own warps' records in shared memory and writes the output; otherwise its share of all steps, and records for the merge.
+template <int HD, int NB, bool I8, bool WHOLE>
 __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeParams p) {
     constexpr int CH = HD / 16;                           // 16-byte pieces per row
     constexpr int RING = KV8_RING<HD, NB>;
@@ -81,12 +101,20 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
     if (p.steps.kv_len && lane < p.steps.B) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.steps.kv_len + lane));
     cwk_pdl_wait();
     GqaList list;
-    const int n = gqa_range(p.steps, lane, list, at);
-    if (n <= 0) {
-        if (warp == 0) gqa_note(p.steps, list, lane);
-        return;
+    int n;
+    if constexpr (WHOLE) {
+        at.b = (int)blockIdx.x / p.steps.groups;
+        at.hg = (int)blockIdx.x % p.steps.groups;
+        at.len = length_of(p.steps, at.b);
+        at.steps = n = (at.len + keys - 1) / keys;
+    } else {
+        n = gqa_range(p.steps, lane, list, at);
+        if (n <= 0) {
+            if (warp == 0) gqa_note(p.steps, list, lane);
+            return;
+        }
+        at.len = length_of(p.steps, at.b);
     }
-    at.len = length_of(p.steps, at.b);
     GqaPlace ld = at;                                     // the step being loaded
     auto head_of = [&](const GqaPlace &x) { return (x.hg / p.parts) * p.hb + wh; };
     auto query = [&](const GqaPlace &x, int col, bool &on) {      // row `col` of the place's queries
@@ -140,7 +168,7 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
     scales(at, ks, vs);
 #pragma unroll
     for (int i = 0; i < RING - 1; i++) load_next();
-    if (warp == 0) gqa_note(p.steps, list, lane);
+    if (!WHOLE && warp == 0) gqa_note(p.steps, list, lane);
     uint32_t bq[QS ? 1 : HD / 16][NB][2];                 // the query rows, as the score MMAs' second operand
     float acc[HD / 16][NB][4];                            // value columns 16 i + 2 lg (+ 1) of query rows 8 nb + 2 lt, + 1
     float m[NB][2], l[NB][2], unit[NB][2];                // unit: what a score MMA's result is multiplied by, besides the key scale
@@ -299,7 +327,9 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
         fresh = at.step + 1 == at.steps;
         if (fresh || s + 1 == n) {                        // the end of what this block has of the sequence's head group: its record
             const int64_t slot = (int64_t)at.b * p.steps.groups + at.hg + blockIdx.x;
-            float *rec = p.rec + (slot * GW + warp) * kv8_record(cols, HD);
+            float *rec = WHOLE ? reinterpret_cast<float *>(smem + warp * (RING + (QS ? 1 : 0)) * KB) : p.rec + (slot * GW + warp) * kv8_record(cols, HD);
+            static_assert(kv8_record(8 * NB, HD) * 4 <= (RING + (QS ? 1 : 0)) * KB, "a record in the place of the ring");
+            if (WHOLE) __syncwarp();                      // every lane has read its last values
 #pragma unroll
             for (int nb = 0; nb < NB; nb++)
 #pragma unroll
@@ -309,6 +339,16 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
                     for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                     const int col = nb * 8 + 2 * lt + x;
                     if (col >= cols) continue;
+                    if (WHOLE && p.hb == GW) {            // the warp has all of the rows' keys
+                        const int tok = at.hg % p.parts * p.per + col / p.group;
+                        if (tok >= p.n) continue;
+                        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+                        uint16_t *dst = p.out + (((int64_t)at.b * p.n + tok) * p.nh + head_of(at) * p.group + col % p.group) * HD + 2 * lg;
+#pragma unroll
+                        for (int i = 0; i < HD / 16; i++)
+                            *reinterpret_cast<uint32_t *>(dst + i * 16) = pack_bf16x2(acc[i][nb][x] * inv, acc[i][nb][2 + x] * inv);
+                        continue;
+                    }
                     float *o = rec + col * HD;
                     if (lg == 0) *reinterpret_cast<float2 *>(rec + cols * HD + col * 2) = make_float2(sum != 0.f ? m[nb][x] : -INFINITY, sum);
 #pragma unroll
@@ -320,6 +360,31 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
         ks = ks_next; vs = vs_next;
     }
     cp_async_wait<0>();
+    if constexpr (WHOLE) {
+        if (p.hb == GW && n > 0) return;
+        __syncthreads();
+        // the warps take the query rows of the block's KV heads in turn; no rows in the cache: zeros
+        const int b = (int)blockIdx.x / p.steps.groups, hg = (int)blockIdx.x % p.steps.groups;
+#pragma unroll 1
+        for (int row = warp; row < p.hb * cols; row += GW) {
+            const int w = row / cols, col = row % cols, tok = hg % p.parts * p.per + col / p.group;
+            if (tok >= p.n) continue;
+            Kv8Sum s[HD / 128];
+            for (int k = w; k < GW && n > 0; k += p.hb) {
+                const float *rec = reinterpret_cast<const float *>(smem + k * (RING + (QS ? 1 : 0)) * KB);
+                const float2 ml = *reinterpret_cast<const float2 *>(rec + cols * HD + col * 2);
+                if (ml.x == -INFINITY) continue;
+#pragma unroll
+                for (int j = 0; j < HD / 128; j++) {
+                    if (ml.x > s[j].M) s[j].raise(ml.x);
+                    s[j].add(exp2f(ml.x - s[j].M), ml.y, *reinterpret_cast<const float4 *>(rec + col * HD + j * 128 + lane * 4));
+                }
+            }
+            uint16_t *dst = p.out + (((int64_t)b * p.n + tok) * p.nh + (hg / p.parts * p.hb + w) * p.group + col % p.group) * HD + lane * 4;
+#pragma unroll
+            for (int j = 0; j < HD / 128; j++) s[j].write(dst + j * 128);
+        }
+    }
 }
 
 // The records of one query row (token x head of sequence b): cnt of them, {m, l} and o of the i-th at ml(i) and o(i).
@@ -338,63 +403,50 @@ struct Kv8Records {
     // slot first + i / ks, warp (i % ks) * hb + kvh % hb
     __device__ __forceinline__ const float *at(int i) const { return base + (ks == 1 ? (int64_t)i * GW : (int64_t)(i / ks) * GW + (i % ks) * hb) * rsz; }
 };
-// Four columns of the records first, first + stride, .., eight records' loads at once; the running maximum as the scores'.
-struct Kv8Sum {
-    float M = -INFINITY, den = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    __device__ __forceinline__ void add(float w, float l, const float4 &v) {
-        den += w * l; o.x += w * v.x; o.y += w * v.y; o.z += w * v.z; o.w += w * v.w;
-    }
-    __device__ __forceinline__ void run(const Kv8Records &r, int column, int first, int stride) {
-        for (int i0 = first; i0 < r.cnt; i0 += 8 * stride) {
-            float2 ml[8];
-            float4 v[8];
+// The records first, first + stride, .., eight records' loads at once; the running maximum as the scores'.
+__device__ __forceinline__ void kv8_add_records(Kv8Sum &s, const Kv8Records &r, int column, int first, int stride) {
+    for (int i0 = first; i0 < r.cnt; i0 += 8 * stride) {
+        float2 ml[8];
+        float4 v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float *at = r.at(min(i0 + j * stride, r.cnt - 1));
-                ml[j] = *reinterpret_cast<const float2 *>(at + r.ml);
-                v[j] = *reinterpret_cast<const float4 *>(at + r.o + column);
-                if (i0 + j * stride >= r.cnt) ml[j].x = -INFINITY;
-            }
-            float to = M;
-#pragma unroll
-            for (int j = 0; j < 8; j++) to = fmaxf(to, ml[j].x);
-            if (to == -INFINITY) continue;
-            const float a = exp2f(M - to);
-            den *= a; o.x *= a; o.y *= a; o.z *= a; o.w *= a;
-            M = to;
-#pragma unroll
-            for (int j = 0; j < 8; j++) add(exp2f(ml[j].x - M), ml[j].y, v[j]);
+        for (int j = 0; j < 8; j++) {
+            const float *at = r.at(min(i0 + j * stride, r.cnt - 1));
+            ml[j] = *reinterpret_cast<const float2 *>(at + r.ml);
+            v[j] = *reinterpret_cast<const float4 *>(at + r.o + column);
+            if (i0 + j * stride >= r.cnt) ml[j].x = -INFINITY;
         }
+        float to = s.M;
+#pragma unroll
+        for (int j = 0; j < 8; j++) to = fmaxf(to, ml[j].x);
+        if (to == -INFINITY) continue;
+        s.raise(to);
+#pragma unroll
+        for (int j = 0; j < 8; j++) s.add(exp2f(ml[j].x - to), ml[j].y, v[j]);
     }
-    __device__ __forceinline__ void write(uint16_t *out) const {
-        const float inv = den != 0.f ? 1.f / den : 0.f;
-        *reinterpret_cast<uint2 *>(out) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-    }
-};
+}
 
 // Few records a row: 256 threads have the rows of a sequence one after another, four columns each. grid (parts of n * nh rows, sequence)
 template <int HD>
-__global__ void __launch_bounds__(256) kv8_merge_few_kernel(const Kv8DecodeParams p, uint16_t *out) {
+__global__ void __launch_bounds__(256) kv8_merge_few_kernel(const Kv8DecodeParams p) {
     const int row = blockIdx.x * (1024 / HD) + threadIdx.x / (HD / 4), column = threadIdx.x % (HD / 4) * 4, b = blockIdx.y;
     cwk_pdl_launch();
     cwk_pdl_wait();
     if (row >= p.n * p.nh) return;
     Kv8Sum s;
-    s.run(Kv8Records(p, HD, b, row / p.nh, row % p.nh), column, 0, 1);
-    s.write(out + ((int64_t)b * p.n * p.nh + row) * HD + column);
+    kv8_add_records(s, Kv8Records(p, HD, b, row / p.nh, row % p.nh), column, 0, 1);
+    s.write(p.out + ((int64_t)b * p.n * p.nh + row) * HD + column);
 }
 // Many: 64 columns of a row to a block, its records dealt out to GROUPS groups of 16 threads: what counts is that all are asked for at
 // once. grid (row, sequence, HD / 64)
 template <int HD, int GROUPS>
-__global__ void __launch_bounds__(16 * GROUPS) kv8_merge_kernel(const Kv8DecodeParams p, uint16_t *out) {
+__global__ void __launch_bounds__(16 * GROUPS) kv8_merge_kernel(const Kv8DecodeParams p) {
     __shared__ float s_m[GROUPS], s_l[GROUPS];
     __shared__ float4 s_o[GROUPS][16];
     const int row = blockIdx.x, b = blockIdx.y, g = threadIdx.x / 16, t = threadIdx.x % 16, column = blockIdx.z * 64 + t * 4;
     cwk_pdl_launch();
     cwk_pdl_wait();
     Kv8Sum s;
-    s.run(Kv8Records(p, HD, b, row / p.nh, row % p.nh), column, g, GROUPS);
+    kv8_add_records(s, Kv8Records(p, HD, b, row / p.nh, row % p.nh), column, g, GROUPS);
     if (t == 0) { s_m[g] = s.M; s_l[g] = s.den; }
     s_o[g][t] = s.o;
     __syncthreads();
@@ -404,14 +456,14 @@ __global__ void __launch_bounds__(16 * GROUPS) kv8_merge_kernel(const Kv8DecodeP
     for (int j = 0; j < GROUPS; j++) all.M = fmaxf(all.M, s_m[j]);
 #pragma unroll
     for (int j = 0; j < GROUPS; j++) all.add(s_m[j] == -INFINITY ? 0.f : exp2f(s_m[j] - all.M), s_l[j], s_o[j][t]);
-    all.write(out + ((int64_t)b * p.n * p.nh + row) * HD + column);
+    all.write(p.out + ((int64_t)b * p.n * p.nh + row) * HD + column);
 }
 
-template <int HD, int NB>
-int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *out) {
+template <int HD, int NB, bool WHOLE>
+int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks) {
     constexpr int SMEM = GW * (KV8_RING<HD, NB> + (KV8_Q_SHARED<HD, NB> ? 1 : 0)) * GK * HD;      // 96 KB
     const bool i8 = type == CWK_KV8_INT8;
-    auto kern = i8 ? kv8_decode_kernel<HD, NB, true> : kv8_decode_kernel<HD, NB, false>;
+    auto kern = i8 ? kv8_decode_kernel<HD, NB, true, WHOLE> : kv8_decode_kernel<HD, NB, false, WHOLE>;
     static bool attr_set[2][16] = {};
     if (!attr_set[i8][ctx->device & 15]) {
         CWK_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
@@ -422,6 +474,7 @@ int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *o
         CWK_CUDA(ctx, cwk_launch_early(kern, dim3(blocks), dim3(32 * GW), SMEM, ctx->stream, p));
         ctx->launches++;
     }
+    if (WHOLE) return CWK_OK;
     // Records per query row; the threads that a group of 16 for every 64 columns of a row makes. Groups as long as there are records for them
     // and the SMs are not filled more than once (37 tokens of 32 heads after 300 rows, 222 blocks, 12 records a row, 1184 rows: 26.8 us with eight
     // groups a row, 15.2 with one).
@@ -430,9 +483,8 @@ int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *o
     if (each > 8 && room >= 4) {
         const int groups = room >= 16 ? 16 : room >= 8 ? 8 : 4;
         CWK_CUDA(ctx, cwk_launch_early(groups == 16 ? kv8_merge_kernel<HD, 16> : groups == 8 ? kv8_merge_kernel<HD, 8> : kv8_merge_kernel<HD, 4>,
-                                       dim3((unsigned)rows, p.steps.B, HD / 64), dim3(16 * groups), 0, ctx->stream, p, (uint16_t *)out));
-    } else CWK_CUDA(ctx, cwk_launch_early(kv8_merge_few_kernel<HD>, dim3((unsigned)((rows + 1024 / HD - 1) / (1024 / HD)), p.steps.B), dim3(256), 0, ctx->stream,
-                                          p, (uint16_t *)out));
+                                       dim3((unsigned)rows, p.steps.B, HD / 64), dim3(16 * groups), 0, ctx->stream, p));
+    } else CWK_CUDA(ctx, cwk_launch_early(kv8_merge_few_kernel<HD>, dim3((unsigned)((rows + 1024 / HD - 1) / (1024 / HD)), p.steps.B), dim3(256), 0, ctx->stream, p));
     ctx->launches++;
     return CWK_OK;
 }
@@ -441,37 +493,47 @@ int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks, void *o
 
 namespace {
 
-// The shape of a pass of the streams over `B` sequences of up to `len` rows.
+// The shape of a pass over `B` sequences of up to `len` rows, and what it takes.
+//
+// Whole: a block for each head group, no records, no merge and its launch. Otherwise equal shares of all steps. By a cost of each side, in us a
+// call replayed, fitted to 1 to 64 sequences of 20 to 700 rows, one and four tokens (and in shares to 580 chunks of 4 to 300 tokens after 0 to
+// 12000 rows); a launch less is worth a microsecond to whoever launches. Whole / shares, 16 heads, 4 KV heads of 256: one sequence of 20 rows
+// 4.7 / 7.8, of 100 9.4 / 7.8; 64 of 60 6.8 / 9.9, of 200 13.5 / 14.9, of 400 21.4 / 17.1; 4 tokens, 64 of 60 10.0 / 16.4.
 struct Kv8Shape {
-    int hb, per, parts, keys, blocks;
-    int64_t groups, steps;            // steps: at most
-    Kv8Shape(int sm_count, int B, int64_t len, int n, int nh, int nkv, int max_blocks) {
+    int hb, per, parts, keys, cols, blocks;
+    int64_t groups;
+    bool whole;
+    double us;
+    Kv8Shape(int sm_count, int B, int64_t len, int n, int nh, int nkv, int hd, int max_blocks) {
         const int group = nh / nkv;
         hb = nkv % 4 == 0 ? 4 : nkv % 2 == 0 ? 2 : 1;
         per = std::min(n, std::max(1, 16 / group));
         parts = (n + per - 1) / per;
         keys = GK * (GW / hb);
+        cols = per * group;
         groups = (int64_t)(nkv / hb) * parts;
-        steps = B * groups * ((len + keys - 1) / keys);
+        const int64_t each = (len + keys - 1) / keys, all = B * groups, steps = all * each, sms = sm_count;
         // as many blocks as there can be steps, at most two per SM
-        blocks = (int)std::min<int64_t>(std::max<int64_t>(1, steps), max_blocks > 0 ? std::min(max_blocks, 2 * sm_count) : 2 * sm_count);
+        blocks = (int)std::min<int64_t>(std::max<int64_t>(1, steps), max_blocks > 0 ? std::min<int64_t>(max_blocks, 2 * sms) : 2 * sms);
+        const bool wide = hd == 256, two = cols > 8;
+        const double turns = (double)((steps + blocks - 1) / blocks), records = (double)blocks * GW * cols * hd * 4e-6;
+        const double shares = (wide ? 6.8 : 6.0) + turns * (two ? (wide ? 3.1 : 1.85) : (wide ? 0.94 : 0.82)) + 0.65 * records;
+        const double one = (double)(((all + 2 * sms - 1) / (2 * sms)) * each) * (two ? (wide ? 2.1 : 1.22) : (wide ? 1.35 : 1.03)) * (all > sms ? 1.3 : 1.0) +
+                           (two ? (wide ? 5.7 : 4.8) : (wide ? 3.9 : 3.2)) + (hb < GW ? 0.7 + 0.3 * hb * cols / GW : 0.0);
+        whole = max_blocks == 0 && all < (1 << 30) && one <= shares + 1.0;
+        us = whole ? one : shares;
+        if (whole) blocks = (int)all;
     }
-    int cols(int group) const { return per * group; }
 };
 
 // Which way a chunk goes. The streams read the codes once for every 16 query rows, every row over all keys; the tensor-core kernel has 128
-// query tokens of a head in a tile, but wants the cache widened and three or four launches. Fitted to 580 chunks of 4 to 300 tokens after 0 to 12000
-// rows, (16, 4), (8, 1), (8, 8), (32, 2), (24, 3) and (16, 2) heads, us a call replayed (mean error 5 to 12 %; the choice costs 1.5 % of the better
-// side's time on average). Streams / tensor cores, 16 heads, 4 KV heads of 256: 4 tokens after 2000 rows 11 / 37, 37 after 2500 28 / 38, 128 after 2000
-// 53 / 41, 64 after 12000 81 / 65; of 128: 64 after 2000 19 / 30, 200 after 12000 122 / 55.
+// query tokens of a head in a tile, but wants the cache widened and three or four launches. Its cost fitted to the same 580 chunks ((16, 4), (8, 1),
+// (8, 8), (32, 2), (24, 3) and (16, 2) heads). Streams / tensor cores, 16 heads, 4 KV heads of 256: 4 tokens after 2000 rows 11 / 37, 37 after
+// 2500 26 / 38, 128 after 2000 45 / 41, 64 after 12000 71 / 65; of 128: 64 after 2000 17 / 30, 200 after 12000 115 / 55.
 bool kv8_streams_sooner(int sm_count, int64_t pos, int n, int nh, int nkv, int hd) {
-    const int group = nh / nkv;
-    if (group > 16) return false;
+    if (nh / nkv > 16) return false;
     const int64_t T = pos + n;
     const bool wide = hd == 256;
-    const Kv8Shape s(sm_count, 1, T, n, nh, nkv, 0);
-    const double turns = (double)((s.steps + s.blocks - 1) / s.blocks), records = (double)s.blocks * GW * s.cols(group) * hd * 4e-6;
-    const double streams = (wide ? 6.8 : 6.0) + turns * (s.cols(group) <= 8 ? (wide ? 0.94 : 0.82) : (wide ? 3.1 : 1.85)) + 0.65 * records;
     // items of 128 tokens x one head, 64 keys a tile; where the longest block has many tiles above an equal share they are dealt out in shares and joined
     const int64_t items = (int64_t)((n + 127) / 128) * nh;
     const auto tiles = [&](int64_t last) { return (last + 63) / 64; };
@@ -481,7 +543,7 @@ bool kv8_streams_sooner(int sm_count, int64_t pos, int n, int nh, int nkv, int h
     const int64_t dealt = std::max(tiles(T), share + idle * tiles(pos + std::min(128, n)) / sm_count);
     const bool shared = dealt > share + 28;
     const double tensor = (wide ? 15.5 : 14.3) + (double)(shared ? share : dealt) * (wide ? 0.64 : 0.54) + (shared ? (wide ? 17.4 : 14.0) : 0.0) + (double)T * nkv * hd * 6 * 0.256e-6;
-    return streams < tensor;
+    return Kv8Shape(sm_count, 1, T, n, nh, nkv, hd, 0).us < tensor;
 }
 
 }  // namespace
@@ -490,19 +552,26 @@ int cwk_kv8_streams(cwk_ctx *ctx, const void *q, const cwk_kv8 &c, const int32_t
                     void *out, int max_blocks) {
     Kv8DecodeParams p{};
     p.q = (const uint16_t *)q; p.k = (const uint8_t *)c.k; p.v = (const uint8_t *)c.v; p.ks = c.k_scale; p.vs = c.v_scale; p.rows = c.rows;
-    const Kv8Shape shape(ctx->sm_count, B, max_kv_len, n, nh, c.nkv, max_blocks);
+    const Kv8Shape shape(ctx->sm_count, B, max_kv_len, n, nh, c.nkv, c.hd, max_blocks);
     const int blocks = shape.blocks;
     p.n = n; p.nh = nh; p.nkv = c.nkv; p.group = nh / c.nkv; p.hb = shape.hb; p.per = shape.per; p.parts = shape.parts;
     p.lb = c.block == 32 ? 5 : c.block == 64 ? 6 : 7;
     p.scale_log2 = scale * 1.4426950408889634f;
     if (shape.groups > 0x7FFFFFFF) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_decode_kv8: too many query tokens");
-    const size_t rec_bytes = (size_t)(B * shape.groups + blocks) * GW * kv8_record(shape.cols(p.group), c.hd) * sizeof(float);
+    p.out = (uint16_t *)out;
+    p.steps = GqaSteps{kv_len, B, (int)shape.groups, shape.keys, kv_len ? (int)c.rows : max_kv_len, nullptr};
+    const bool two = shape.cols > 8;
+    if (shape.whole) {
+        if (c.hd == 256) return two ? launch<256, 2, true>(ctx, p, c.type, blocks) : launch<256, 1, true>(ctx, p, c.type, blocks);
+        return two ? launch<128, 2, true>(ctx, p, c.type, blocks) : launch<128, 1, true>(ctx, p, c.type, blocks);
+    }
+    const size_t rec_bytes = (size_t)(B * shape.groups + blocks) * GW * kv8_record(shape.cols, c.hd) * sizeof(float);
     const int s = cwk_reserve_scratch(ctx, rec_bytes + (size_t)B * shape.groups * sizeof(int2));
     if (s != CWK_OK) return s;
     p.rec = ctx->scratch;
-    p.steps = GqaSteps{kv_len, B, (int)shape.groups, shape.keys, kv_len ? (int)c.rows : max_kv_len, (int2 *)((uint8_t *)ctx->scratch + rec_bytes)};
-    if (p.per * p.group > 8) return c.hd == 256 ? launch<256, 2>(ctx, p, c.type, blocks, out) : launch<128, 2>(ctx, p, c.type, blocks, out);
-    return c.hd == 256 ? launch<256, 1>(ctx, p, c.type, blocks, out) : launch<128, 1>(ctx, p, c.type, blocks, out);
+    p.steps.meta = (int2 *)((uint8_t *)ctx->scratch + rec_bytes);
+    if (c.hd == 256) return two ? launch<256, 2, false>(ctx, p, c.type, blocks) : launch<256, 1, false>(ctx, p, c.type, blocks);
+    return two ? launch<128, 2, false>(ctx, p, c.type, blocks) : launch<128, 1, false>(ctx, p, c.type, blocks);
 }
 
 // mla_prefill_attn.cu
