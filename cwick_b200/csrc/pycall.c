@@ -78,10 +78,15 @@ WRAP(cwk_gqa_decode_kv8, 11, {
     const int nh = i32(a[7]); const float scale = f32(a[8]); void *out = ptr(a[9]); const int splits = i32(a[10]);
     RUN(cwk_gqa_decode_kv8(c, q, cache, len, max_len, B, n_, nh, scale, out, splits));
 })
+WRAP(cwk_gqa_prefill_kv8, 9, {
+    cwk_ctx *c = ptr(a[0]); void *q = ptr(a[1]), *cache = ptr(a[2]); const int slot = i32(a[3]); const int64_t pos = i64(a[4]);
+    const int n_ = i32(a[5]), nh = i32(a[6]); const float scale = f32(a[7]); void *out = ptr(a[8]);
+    RUN(cwk_gqa_prefill_kv8(c, q, cache, slot, pos, n_, nh, scale, out));
+})
 
 static PyMethodDef methods[] = {
 #define M(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, NULL}
     M(cwk_mla_decode), M(cwk_gqa_decode), M(cwk_dsa_select), M(cwk_gdn_scan), M(cwk_kv8_store), M(cwk_kv8_load),
-    M(cwk_gqa_qk_prep_kv8), M(cwk_gqa_decode_kv8), {NULL, NULL, 0, NULL}};
+    M(cwk_gqa_qk_prep_kv8), M(cwk_gqa_decode_kv8), M(cwk_gqa_prefill_kv8), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_pycall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__pycall(void) { return PyModule_Create(&module); }

@@ -20,12 +20,25 @@ def _bf16(t):
     return t
 
 
+_I32 = torch.int32
+_ROWS = {torch.bfloat16: 0, torch.float32: 1}
+
+
 def _i32(t, B):
     """The address of an int32 [B] cuda tensor, or None."""
     if t is None:
         return None
-    assert t.dtype == torch.int32 and t.is_cuda and t.is_contiguous() and t.shape == (B,)
+    assert t.dtype is _I32 and t.is_cuda and t.is_contiguous() and t.dim() == 1 and t.numel() == B
     return t.data_ptr()
+
+
+def _kv8_rows(cache, device, k, v):
+    """(B, n, 1 for f32 and 0 for bf16) of K and V rows [B][n][nkv][hd]."""
+    shape, dtype = k.shape, k.dtype
+    B, n, nkv, hd = shape
+    assert v.shape == shape and nkv == cache.nkv and hd == cache.hd and v.dtype is dtype and dtype in _ROWS
+    assert k.is_contiguous() and v.is_contiguous() and k.is_cuda and v.is_cuda and cache.device == device
+    return B, n, _ROWS[dtype]
 
 
 class Kv8Cache:
@@ -62,8 +75,8 @@ class Attn:
         # the calls of a decode step: plain integers and floats in, status out
         self._mla_decode, self._gqa_decode, self._dsa_select, self._gdn_scan = (
             _lib.fast(self.lib, "cwk_" + n) for n in ("mla_decode", "gqa_decode", "dsa_select", "gdn_scan"))
-        self._kv8_store, self._kv8_load, self._gqa_qk_prep_kv8, self._gqa_decode_kv8 = (
-            _lib.fast(self.lib, "cwk_" + n) for n in ("kv8_store", "kv8_load", "gqa_qk_prep_kv8", "gqa_decode_kv8"))
+        self._kv8_store, self._kv8_load, self._gqa_qk_prep_kv8, self._gqa_decode_kv8, self._gqa_prefill_kv8 = (
+            _lib.fast(self.lib, "cwk_" + n) for n in ("kv8_store", "kv8_load", "gqa_qk_prep_kv8", "gqa_decode_kv8", "gqa_prefill_kv8"))
 
     # ---- MLA ---------------------------------------------------------------
     def mla_decode(self, q, cache, kv_len, max_kv_len=None, sel=None, scale=None, seq_stride=None,
@@ -207,24 +220,19 @@ class Attn:
     # ---- GQA cache held in 8 bits ----------------------------------------------------
     def kv8_store(self, cache, k, v, pos, count=None):
         """Rows pos[b] .. of slot b from k, v [B][n][nkv][hd] (bf16 or f32); pos, count int32 [B] cuda (count None: n rows each)."""
-        B, n = k.shape[:2]
-        assert cache.device == self.device and k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.is_contiguous() and v.is_contiguous()
-        assert k.shape == v.shape == (B, n, cache.nkv, cache.hd)
-        st = self._kv8_store(self.ctx.address, cache.address, k.data_ptr(), v.data_ptr(), 1 if k.dtype == torch.float32 else 0,
-                             _i32(pos, B), _i32(count, B), B, n)
+        B, n, f32 = _kv8_rows(cache, self.device, k, v)
+        st = self._kv8_store(self.ctx.address, cache.address, k.data_ptr(), v.data_ptr(), f32, _i32(pos, B), _i32(count, B), B, n)
         if st:
             self.ctx.check(st)
 
     def kv8_load(self, cache, pos, n, count=None, dtype=torch.bfloat16, out=None):
         """Rows pos[b] + 0 .. n - 1 of slot b as values: (K, V), each [B][n][nkv][hd]; rows from count[b] on are not written."""
-        B = pos.shape[0]
         if out is None:
-            out = tuple(torch.empty(B, n, cache.nkv, cache.hd, dtype=dtype, device=cache.k.device) for _ in range(2))
+            out = tuple(torch.empty(pos.shape[0], n, cache.nkv, cache.hd, dtype=dtype, device=cache.k.device) for _ in range(2))
         k, v = out
-        assert cache.device == self.device and k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.is_contiguous() and v.is_contiguous()
-        assert k.shape == v.shape == (B, n, cache.nkv, cache.hd)
-        st = self._kv8_load(self.ctx.address, cache.address, _i32(pos, B), _i32(count, B), B, n, k.data_ptr(), v.data_ptr(),
-                            1 if k.dtype == torch.float32 else 0)
+        B, rows, f32 = _kv8_rows(cache, self.device, k, v)
+        assert rows == n
+        st = self._kv8_load(self.ctx.address, cache.address, _i32(pos, B), _i32(count, B), B, n, k.data_ptr(), v.data_ptr(), f32)
         if st:
             self.ctx.check(st)
         return k, v
@@ -232,10 +240,11 @@ class Attn:
     def gqa_qk_prep_kv8(self, cache, qg, k, v, q_norm, k_norm, eps, rot, theta, pos, count=None, q_out=None):
         """Norms, rotation and the cache's new rows in one pass (cwk_gqa_qk_prep_kv8): qg f32 [B][n][nh][2*hd], k, v f32 [B][n][nkv][hd].
         Returns q bf16 [B][n][nh][hd]; rows from count[b] on are not written."""
-        B, n, nh, _ = qg.shape
-        for t in (qg, k, v, q_norm, k_norm):
-            assert t.dtype == torch.float32 and t.is_contiguous()
-        assert cache.device == self.device and qg.shape[3] == 2 * cache.hd and k.shape == v.shape == (B, n, cache.nkv, cache.hd) and q_norm.numel() == k_norm.numel() == cache.hd
+        B, n, f32 = _kv8_rows(cache, self.device, k, v)
+        nh = qg.shape[2]
+        assert f32 and qg.shape == (B, n, nh, 2 * cache.hd) and q_norm.numel() == k_norm.numel() == cache.hd
+        for t in (qg, q_norm, k_norm):
+            assert t.dtype is torch.float32 and t.is_contiguous() and t.is_cuda
         if q_out is None:
             q_out = torch.empty(B, n, nh, cache.hd, dtype=torch.bfloat16, device=qg.device)
         assert _bf16(q_out).shape == (B, n, nh, cache.hd)
@@ -248,15 +257,19 @@ class Attn:
     def gqa_decode_kv8(self, q, cache, kv_len, scale=None, max_kv_len=None, n_splits=0, out=None):
         """q bf16 [B][nh][hd], or [B][n][nh][hd] for n query tokens per sequence; kv_len int32 [B], those tokens' rows included."""
         _bf16(q)
-        B, n, nh, hd = q.shape if q.dim() == 4 else (q.shape[0], 1, *q.shape[1:])
+        if q.dim() == 4:
+            B, n, nh, hd = q.shape
+        else:
+            (B, nh, hd), n = q.shape, 1
         assert hd == cache.hd and cache.device == self.device
         if scale is None:
-            scale = 1.0 / math.sqrt(hd)
+            scale = hd ** -0.5
         if max_kv_len is None:
             max_kv_len = int(kv_len.max().item())
         if out is None:
             out = torch.empty_like(q)
-        assert _bf16(out).shape == q.shape
+        else:
+            assert _bf16(out).shape == q.shape
         st = self._gqa_decode_kv8(self.ctx.address, q.data_ptr(), cache.address, _i32(kv_len, B), max_kv_len, B, n, nh, scale, out.data_ptr(), n_splits)
         if st:
             self.ctx.check(st)
@@ -268,8 +281,10 @@ class Attn:
         n, nh, hd = Q.shape
         assert hd == cache.hd and cache.device == self.device
         out = torch.empty_like(Q)
-        self.ctx.check(self.lib.cwk_gqa_prefill_kv8(self.ctx.h, _p(Q), cache.address, slot, pos, n, nh, 1.0 / math.sqrt(hd) if scale is None else scale,
-                                                    _p(out)))
+        st = self._gqa_prefill_kv8(self.ctx.address, Q.data_ptr(), cache.address, slot, pos, n, nh, hd ** -0.5 if scale is None else scale,
+                                   out.data_ptr())
+        if st:
+            self.ctx.check(st)
         return out
 
     # ---- FP8 projection ------------------------------------------------------------

@@ -44,7 +44,7 @@ def test_refusals_without_a_device(change, want):
     assert set(calls(L, None)) == {lib.ERR_ARGUMENT}
 
 
-@pytest.mark.parametrize("name", ["cwk_kv8_store", "cwk_kv8_load", "cwk_gqa_qk_prep_kv8", "cwk_gqa_decode_kv8"])
+@pytest.mark.parametrize("name", ["cwk_kv8_store", "cwk_kv8_load", "cwk_gqa_qk_prep_kv8", "cwk_gqa_decode_kv8", "cwk_gqa_prefill_kv8"])
 def test_a_decode_steps_calls_are_in_the_compiled_binding(name):
     L = lib.load()
     fn = lib.fast(L, name)
