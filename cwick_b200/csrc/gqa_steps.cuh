@@ -27,7 +27,7 @@ __device__ __forceinline__ int steps_of(const GqaSteps &p, int b) { return b < p
 // copies were 4 us of a step of 16 sequences).
 struct GqaList {
     int mine, upto;
-    int64_t total;
+    int64_t total, lo, hi;                    // lo, hi: the block's steps
 };
 __device__ __forceinline__ void gqa_round(const GqaSteps &p, int b0, int lane, GqaList &s) {
     s.mine = steps_of(p, b0 + lane);
@@ -74,8 +74,9 @@ template <class U> __device__ __forceinline__ U gqa_from(U total, U g) {
     return g >= G ? total : G == total ? g : total * g / G;
 }
 template <class U>
-__device__ __forceinline__ int gqa_share(const GqaSteps &p, const GqaList &s, int lane, GqaPlace &at) {
+__device__ __forceinline__ int gqa_share(const GqaSteps &p, GqaList &s, int lane, GqaPlace &at) {
     const U total = (U)s.total, lo = gqa_from<U>(total, blockIdx.x), hi = gqa_from<U>(total, blockIdx.x + 1);
+    s.lo = lo; s.hi = hi;
     gqa_walk<U>(p, s, lane, [&](int b0, int mine, U s0) {
         const uint32_t who = __ballot_sync(0xffffffffu, mine > 0 && s0 <= lo && lo < s0 + (U)mine * (U)p.groups && lo < hi);
         if (who) {
@@ -96,6 +97,7 @@ __device__ __forceinline__ int gqa_range(const GqaSteps &p, int lane, GqaList &s
         s.total = (int64_t)s.mine * p.groups;
         if (s.total * (gridDim.x + 1) < (1ll << 32)) {
             const uint32_t lo = gqa_from<uint32_t>((uint32_t)s.total, blockIdx.x), hi = gqa_from<uint32_t>((uint32_t)s.total, blockIdx.x + 1);
+            s.lo = lo; s.hi = hi;
             at.steps = s.mine;
             at.hg = p.groups == 1 || lo == hi ? 0 : lo / (uint32_t)s.mine;
             at.step = (int)lo - at.hg * s.mine;
@@ -110,7 +112,7 @@ __device__ __forceinline__ int gqa_range(const GqaSteps &p, int lane, GqaList &s
 // are numbered by head group plus block: one of the two grows from record to record) and their number.
 template <class U>
 __device__ __forceinline__ void gqa_note_as(const GqaSteps &p, const GqaList &s, int lane) {
-    const U total = (U)s.total, nhg = p.groups, G = gqa_blocks(total), g = blockIdx.x, lo = gqa_from<U>(total, g), hi = gqa_from<U>(total, g + 1);
+    const U total = (U)s.total, nhg = p.groups, G = gqa_blocks(total), g = blockIdx.x, lo = (U)s.lo, hi = (U)s.hi;
     gqa_walk<U>(p, s, lane, [&](int b0, int mine, U s0) {
         const int b = b0 + lane;
         if (b >= p.B) return;
@@ -118,10 +120,10 @@ __device__ __forceinline__ void gqa_note_as(const GqaSteps &p, const GqaList &s,
             if (s0 > 0 ? (lo < s0 && s0 <= hi) : g == 0)
                 for (int h = 0; h < p.groups; h++) p.meta[b * p.groups + h] = make_int2(0, 0);
         } else if (s0 < hi && s0 + (U)mine * nhg > lo) {
-            const U h0 = lo > s0 ? (lo - s0 + mine - 1) / (U)mine : 0;                     // first head group that begins here
+            const U h0 = lo <= s0 ? 0 : nhg == 1 ? 1 : (lo - s0 + mine - 1) / (U)mine;      // first head group that begins here
 #pragma unroll 1
             for (U h = h0; h < nhg && s0 + h * mine < hi; h++) {
-                const U last = s0 + (h + 1) * mine, g1 = G == total ? last - 1 : (last * G - 1) / total;      // the block with its last step
+                const U last = s0 + (h + 1) * mine, g1 = last <= hi ? g : G == total ? last - 1 : (last * G - 1) / total;      // the block with its last step
                 p.meta[b * p.groups + (int)h] = make_int2(b * p.groups + (int)(h + g), (int)(g1 - g + 1));
             }
         }

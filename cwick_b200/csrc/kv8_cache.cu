@@ -6,6 +6,7 @@
 // their RMS norm and rotation (src/q35_model.c:112-122, :144-153, :459-477), and query heads the same on blocks of their own.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kv8.cuh"
 
@@ -13,26 +14,27 @@ namespace {
 
 enum { SRC_BF16 = 0, SRC_F32 = 1 };
 
-struct Kv8WriteParams {
+struct Kv8StoreParams {
     const void *k, *v;                         // [B][n][nkv][hd]
     const int32_t *pos, *count;                // [B]; count NULL: n
     uint8_t *kc, *vc, *ks, *vs;
     int64_t rows;                              // per slot
     int B, n, nkv, lb;                         // block = 1 << lb
     int window;                                // blocks that n rows can touch
-    // preparation
+};
+struct Kv8PrepParams : Kv8StoreParams {
+    int nh, rot, heads;                        // heads: query heads per warp
+    float eps;
     const float *qg, *q_norm, *k_norm;
     uint16_t *q_out;
-    int nh, rot;
-    float eps;
     int64_t tasks;                             // K and V tasks; the blocks behind them have query rows
-    int heads;                                 // query heads per warp
-    double freq_hi[16], freq_lo[8];            // angle per position of pair i: freq_hi[i / 8] * freq_lo[i % 8]
+    double octaves;                            // angle per position of pair i: 2^(-i * octaves)
 };
+static_assert(sizeof(Kv8StoreParams) <= 128, "kernel parameters: more than 128 bytes of them come later");
 constexpr int KQ_HEADS = 8;                    // most query heads of a warp
 
 // new rows of slot b: positions pos .. pos + the result - 1, all inside the slot
-__device__ __forceinline__ int new_rows(const Kv8WriteParams &p, int b, int64_t &pos) {
+__device__ __forceinline__ int new_rows(const Kv8StoreParams &p, int b, int64_t &pos) {
     pos = p.pos[b];
     const int64_t c = p.count ? min(p.count[b], p.n) : p.n;
     return pos < 0 ? 0 : (int)max((int64_t)0, min(c, p.rows - pos));
@@ -84,14 +86,14 @@ __device__ __forceinline__ bool subnormal(float x) {
 }
 
 // The angle of pair i per position.
-__device__ __forceinline__ double frequency(const Kv8WriteParams &p, int i) { return p.freq_hi[i >> 3] * p.freq_lo[i & 7]; }
+__device__ __forceinline__ double frequency(double octaves, int i) { return exp2(-(double)i * octaves); }
 // cos and sin of the angles at positions pos .. pos + rows - 1 by a warp, [rows][pairs]: the angle taken into [-pi, pi] in double, then
 // rounded to float (2^-22); the sum with 1.5 * 2^52 is the nearest whole number of turns. (Not unrolled: the copies of the code that
 // forms a cosine would not stay in the instruction cache.)
-__device__ __forceinline__ void angles(const Kv8WriteParams &p, int pairs, int64_t pos, int rows, int lane, float2 *cs) {
+__device__ __forceinline__ void angles(double octaves, int pairs, int64_t pos, int rows, int lane, float2 *cs) {
 #pragma unroll 1
     for (int i = lane; i < pairs; i += 32) {
-        const double f = frequency(p, i);
+        const double f = frequency(octaves, i);
 #pragma unroll 1
         for (int r = 0; r < rows; r++) {
             const double a = (double)(pos + r) * f, turns = (a * 0.15915494309189533577 + 6755399441055744.0) - 6755399441055744.0;
@@ -103,12 +105,12 @@ __device__ __forceinline__ void angles(const Kv8WriteParams &p, int pairs, int64
     __syncwarp();
 }
 // the same of one position in double
-__device__ __forceinline__ void angles(const Kv8WriteParams &p, int pairs, int64_t pos, int lane, double2 *cs) {
+__device__ __forceinline__ void angles(double octaves, int pairs, int64_t pos, int lane, double2 *cs) {
     __syncwarp();
 #pragma unroll 1
     for (int i = lane; i < pairs; i += 32) {
         double c, s;
-        sincos((double)pos * frequency(p, i), &s, &c);
+        sincos((double)pos * frequency(octaves, i), &s, &c);
         cs[i] = make_double2(c, s);
     }
     __syncwarp();
@@ -236,18 +238,18 @@ __device__ __forceinline__ void rescale(uint8_t *codes, int64_t ld, int lead, in
 
 // V: values of a row per lane (head dim / 32); ROWS: rows of a warp. PREP: f32 rows, keys normed and rotated; blocks from p.tasks on have
 // query rows.
-template <int V, int SRC, bool I8, bool PREP, int ROWS>
-__global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel(const __grid_constant__ Kv8WriteParams p) {
+template <int V, int SRC, bool I8, class PARAMS, int ROWS>
+__global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel(const __grid_constant__ PARAMS p) {
+    constexpr bool PREP = std::is_same<PARAMS, Kv8PrepParams>::value;
     constexpr int HD = 32 * V;
     extern __shared__ double2 s_cs[];                      // PREP: of a warp, [ROWS][rot / 2] cos and sin in float, or [rot / 2] in double
     __shared__ uint32_t s_max[16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    const int pairs = p.rot / 2;
-    float2 *csf = reinterpret_cast<float2 *>(s_cs) + warp * ROWS * pairs;
-    double2 *cs = reinterpret_cast<double2 *>(csf);        // (one of them at a time)
     cwk_pdl_launch();
     cwk_pdl_wait();
-    if (PREP && blockIdx.x >= p.tasks) {
+    if constexpr (PREP) if (blockIdx.x >= p.tasks) {
+        const int pairs = p.rot / 2;
+        float2 *csf = reinterpret_cast<float2 *>(s_cs) + warp * ROWS * pairs;
         // ---- query rows: a warp has `heads` heads of one token
         const int parts = (p.nh + p.heads - 1) / p.heads;
         const int64_t id = ((int64_t)blockIdx.x - p.tasks) * warps + warp, t = id / parts;
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
             if (i < heads) x[i].load(p.qg, (t * p.nh + h0 + i) * 2, lane);      // rows [q | gate] of 2 * hd
         int64_t pos;
         if (j >= new_rows(p, b, pos)) return;
-        angles(p, pairs, pos + j, 1, lane, csf);
+        angles(p.octaves, pairs, pos + j, 1, lane, csf);
         float w1[V];
 #pragma unroll
         for (int i = 0; i < V; i++) w1[i] = 1.f + w[i];
@@ -321,7 +323,10 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
 #pragma unroll
     for (int i = 0; i < ROWS; i++)
         if (i < mine) x[i].load(src, row + i * p.nkv, lane);
-    if (PREP && !is_v) {
+    if constexpr (PREP) if (!is_v) {
+        const int pairs = p.rot / 2;
+        float2 *csf = reinterpret_cast<float2 *>(s_cs) + warp * ROWS * pairs;
+        double2 *cs = reinterpret_cast<double2 *>(csf);    // (one of them at a time)
         // ---- keys. A code is that of the value in 64 bits, formed in float: where a float's error could change the code (or the
         // exponent), the row (or the largest magnitude) is formed again in double. That is one row in thirty or less, and double, with its
         // conversions, is some eight times the work: 512 tokens 20 us with all rows in double.
@@ -341,13 +346,13 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
             if (some)                                      // (an ordinary row has none)
 #pragma unroll
                 for (int i = 0; i < V; i++) x64[i] = (double)z[i];
-            angles(p, pairs, lo + first + r, lane, cs);
+            angles(p.octaves, pairs, lo + first + r, lane, cs);
             norm_rotate<V, double>(x64, rsqrt(warp_sum(squares<V, double>(x64)) / (double)HD + (double)p.eps), w1, p.rot, lane, cs, y);
         };
         float y[ROWS][V];
         uint32_t amax = 0;
         bool unsure = false;
-        angles(p, pairs, lo + first, max(mine, 0), lane, csf);
+        angles(p.octaves, pairs, lo + first, max(mine, 0), lane, csf);
         {
             float w1[V];
 #pragma unroll
@@ -531,15 +536,16 @@ int launch_read(cwk_ctx *ctx, const Kv8ReadParams &p, int hd, bool i8, bool f32)
     return CWK_OK;
 }
 
-template <int V, int SRC, bool PREP, int ROWS>
-int launch_write_rows(cwk_ctx *ctx, Kv8WriteParams &p, int type) {
+template <int V, int SRC, int ROWS, class PARAMS>
+int launch_write_rows(cwk_ctx *ctx, PARAMS &p, int type) {
     const int block = 1 << p.lb, warps = (std::min(block, p.n) + ROWS - 1) / ROWS;
     p.window = (int)(((int64_t)p.n + block - 2) / block + 1);
-    p.tasks = (int64_t)2 * p.B * p.window * p.nkv;
-    int64_t blocks = p.tasks;
+    const int64_t tasks = (int64_t)2 * p.B * p.window * p.nkv;
+    int64_t blocks = tasks;
     size_t smem = 0;
-    auto kern = type == CWK_KV8_INT8 ? kv8_write_kernel<V, SRC, true, PREP, ROWS> : kv8_write_kernel<V, SRC, false, PREP, ROWS>;
-    if (PREP) {
+    auto kern = type == CWK_KV8_INT8 ? kv8_write_kernel<V, SRC, true, PARAMS, ROWS> : kv8_write_kernel<V, SRC, false, PARAMS, ROWS>;
+    if constexpr (std::is_same<PARAMS, Kv8PrepParams>::value) {
+        p.tasks = tasks;
         p.heads = p.n * (int64_t)p.B * p.nh <= 2048 ? 1 : KQ_HEADS;      // query heads that share a token's angles and are on their way together; few rows: a warp each
         blocks += ((int64_t)p.B * p.n * ((p.nh + p.heads - 1) / p.heads) + warps - 1) / warps;
         smem = (size_t)(p.rot / 2) * warps * ROWS * sizeof(float2);      // 128 KB at most (32 KB for 64 values in blocks of 128 rows)
@@ -554,12 +560,14 @@ int launch_write_rows(cwk_ctx *ctx, Kv8WriteParams &p, int type) {
     return CWK_OK;
 }
 // Rows of a warp: eight, and four for the preparation of shorter blocks, whose keys go from row to row.
-template <int V, int SRC, bool PREP>
-int launch_write(cwk_ctx *ctx, Kv8WriteParams &p, int type) {
-    return p.lb == 7 || !PREP ? launch_write_rows<V, SRC, PREP, 8>(ctx, p, type) : launch_write_rows<V, SRC, PREP, 4>(ctx, p, type);
+template <int V, int SRC>
+int launch_write(cwk_ctx *ctx, Kv8StoreParams &p, int type) { return launch_write_rows<V, SRC, 8>(ctx, p, type); }
+template <int V, int SRC>
+int launch_write(cwk_ctx *ctx, Kv8PrepParams &p, int type) {
+    return p.lb == 7 ? launch_write_rows<V, SRC, 8>(ctx, p, type) : launch_write_rows<V, SRC, 4>(ctx, p, type);
 }
 
-void describe(Kv8WriteParams &p, const cwk_kv8 *c, const void *k, const void *v, const int32_t *pos, const int32_t *count, int B, int n) {
+void describe(Kv8StoreParams &p, const cwk_kv8 *c, const void *k, const void *v, const int32_t *pos, const int32_t *count, int B, int n) {
     p.k = k; p.v = v; p.pos = pos; p.count = count; p.B = B; p.n = n; p.nkv = c->nkv; p.lb = log2_of(c->block); p.rows = c->rows;
     p.kc = (uint8_t *)c->k; p.vc = (uint8_t *)c->v; p.ks = c->k_scale; p.vs = c->v_scale;
 }
@@ -596,11 +604,11 @@ int cwk_kv8_store(cwk_ctx *ctx, const cwk_kv8 *c, const void *k, const void *v, 
     if (B <= 0 || n <= 0 || B > c->slots) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "kv8_store: bad dimensions (%d slots, %d rows)", B, n);
     if (!aligned(k, v)) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "kv8_store: pointers must be 16-byte aligned");
     CWK_CUDA(ctx, cudaSetDevice(ctx->device));
-    Kv8WriteParams p{};
+    Kv8StoreParams p{};
     describe(p, c, k, v, pos, count, B, n);
     CwkKernelTimer timer(ctx);
-    if (c->hd == 256) return f32 ? launch_write<8, SRC_F32, false>(ctx, p, c->type) : launch_write<8, SRC_BF16, false>(ctx, p, c->type);
-    return f32 ? launch_write<4, SRC_F32, false>(ctx, p, c->type) : launch_write<4, SRC_BF16, false>(ctx, p, c->type);
+    if (c->hd == 256) return f32 ? launch_write<8, SRC_F32>(ctx, p, c->type) : launch_write<8, SRC_BF16>(ctx, p, c->type);
+    return f32 ? launch_write<4, SRC_F32>(ctx, p, c->type) : launch_write<4, SRC_BF16>(ctx, p, c->type);
 }
 
 int cwk_kv8_load(cwk_ctx *ctx, const cwk_kv8 *c, const int32_t *pos, const int32_t *count, int B, int n, void *k, void *v, int f32) {
@@ -628,15 +636,12 @@ int cwk_gqa_qk_prep_kv8(cwk_ctx *ctx, const float *qg, const float *k, const flo
     if (!aligned(k, v) || !aligned(qg, q_out) || !aligned(q_norm, k_norm))
         return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_qk_prep_kv8: pointers must be 16-byte aligned");
     CWK_CUDA(ctx, cudaSetDevice(ctx->device));
-    Kv8WriteParams p{};
+    Kv8PrepParams p{};
     describe(p, c, k, v, pos, count, B, n);
     p.qg = qg; p.q_norm = q_norm; p.k_norm = k_norm; p.q_out = (uint16_t *)q_out; p.nh = nh; p.rot = rot; p.eps = eps;
-    if (rot > 0) {
-        for (int i = 0; i < 16; i++) p.freq_hi[i] = pow(theta, -16.0 * i / rot);
-        for (int i = 0; i < 8; i++) p.freq_lo[i] = pow(theta, -2.0 * i / rot);
-    }
+    p.octaves = rot > 0 ? 2.0 * log2(theta) / rot : 0.0;
     CwkKernelTimer timer(ctx);
-    return c->hd == 256 ? launch_write<8, SRC_F32, true>(ctx, p, c->type) : launch_write<4, SRC_F32, true>(ctx, p, c->type);
+    return c->hd == 256 ? launch_write<8, SRC_F32>(ctx, p, c->type) : launch_write<4, SRC_F32>(ctx, p, c->type);
 }
 
 }  // extern "C"

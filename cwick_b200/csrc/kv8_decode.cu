@@ -28,13 +28,17 @@ struct Kv8DecodeParams {
     const uint16_t *q;                // bf16 [B][n][nh][hd]
     const uint8_t *k, *v, *ks, *vs;
     int64_t rows;                     // per slot
-    int n, nh, nkv, group, hb, lb;    // hb: KV heads a block works on at once (4, 2 or 1); block = 1 << lb
-    int per, parts;                   // query tokens whose heads share the MMA columns; parts = ceil(n / per)
+    int n, nkv, parts;                // parts = ceil(n / per)
+    uint8_t group, hb, lb, per;       // hb: KV heads a block works on at once (4, 2 or 1); block = 1 << lb; per: query tokens whose heads share the MMA columns
     float scale_log2;
     uint16_t *out;                    // bf16 [B][n][nh][hd]
     float *rec;                       // [slot][warp]: o [per * group][hd], then {m, l} [per * group]
+    __host__ __device__ int nh() const { return nkv * group; }
     GqaSteps steps;                   // groups: (nkv / hb) * parts, the parts of the same keys next to each other; keys: GK * (GW / hb)
 };
+
+// (Parameters of more than 128 bytes come later: with eight more a step of one sequence of 4096 rows took 9.3 us instead of 8.2.)
+static_assert(sizeof(Kv8DecodeParams) <= 128, "kernel parameters");
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -120,7 +124,7 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
     auto query = [&](const GqaPlace &x, int col, bool &on) {      // row `col` of the place's queries
         const int tok = x.hg % p.parts * p.per + col / p.group;
         on = col < cols && tok < p.n;
-        return p.q + (((int64_t)x.b * p.n + tok) * p.nh + head_of(x) * p.group + col % p.group) * HD;
+        return p.q + ((((int64_t)x.b * p.n + tok) * p.nkv + head_of(x)) * p.group + col % p.group) * HD;
     };
     {   // on their way while the first copies are asked for
         bool on;
@@ -326,8 +330,9 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
         }
         fresh = at.step + 1 == at.steps;
         if (fresh || s + 1 == n) {                        // the end of what this block has of the sequence's head group: its record
-            const int64_t slot = (int64_t)at.b * p.steps.groups + at.hg + blockIdx.x;
-            float *rec = WHOLE ? reinterpret_cast<float *>(smem + warp * (RING + (QS ? 1 : 0)) * KB) : p.rec + (slot * GW + warp) * kv8_record(cols, HD);
+            float *rec;
+            if constexpr (WHOLE) rec = reinterpret_cast<float *>(smem + warp * (RING + (QS ? 1 : 0)) * KB);
+            else rec = p.rec + (((int64_t)at.b * p.steps.groups + at.hg + blockIdx.x) * GW + warp) * kv8_record(cols, HD);
             static_assert(kv8_record(8 * NB, HD) * 4 <= (RING + (QS ? 1 : 0)) * KB, "a record in the place of the ring");
             if (WHOLE) __syncwarp();                      // every lane has read its last values
 #pragma unroll
@@ -343,7 +348,7 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
                         const int tok = at.hg % p.parts * p.per + col / p.group;
                         if (tok >= p.n) continue;
                         const float inv = sum != 0.f ? 1.f / sum : 0.f;
-                        uint16_t *dst = p.out + (((int64_t)at.b * p.n + tok) * p.nh + head_of(at) * p.group + col % p.group) * HD + 2 * lg;
+                        uint16_t *dst = p.out + (((int64_t)at.b * p.n + tok) * p.nh() + head_of(at) * p.group + col % p.group) * HD + 2 * lg;
 #pragma unroll
                         for (int i = 0; i < HD / 16; i++)
                             *reinterpret_cast<uint32_t *>(dst + i * 16) = pack_bf16x2(acc[i][nb][x] * inv, acc[i][nb][2 + x] * inv);
@@ -380,7 +385,7 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
                     s[j].add(exp2f(ml.x - s[j].M), ml.y, *reinterpret_cast<const float4 *>(rec + col * HD + j * 128 + lane * 4));
                 }
             }
-            uint16_t *dst = p.out + (((int64_t)b * p.n + tok) * p.nh + (hg / p.parts * p.hb + w) * p.group + col % p.group) * HD + lane * 4;
+            uint16_t *dst = p.out + (((int64_t)b * p.n + tok) * p.nh() + (hg / p.parts * p.hb + w) * p.group + col % p.group) * HD + lane * 4;
 #pragma unroll
             for (int j = 0; j < HD / 128; j++) s[j].write(dst + j * 128);
         }
@@ -431,10 +436,10 @@ __global__ void __launch_bounds__(256) kv8_merge_few_kernel(const Kv8DecodeParam
     const int row = blockIdx.x * (1024 / HD) + threadIdx.x / (HD / 4), column = threadIdx.x % (HD / 4) * 4, b = blockIdx.y;
     cwk_pdl_launch();
     cwk_pdl_wait();
-    if (row >= p.n * p.nh) return;
+    if (row >= p.n * p.nh()) return;
     Kv8Sum s;
-    kv8_add_records(s, Kv8Records(p, HD, b, row / p.nh, row % p.nh), column, 0, 1);
-    s.write(p.out + ((int64_t)b * p.n * p.nh + row) * HD + column);
+    kv8_add_records(s, Kv8Records(p, HD, b, row / p.nh(), row % p.nh()), column, 0, 1);
+    s.write(p.out + ((int64_t)b * p.n * p.nh() + row) * HD + column);
 }
 // Many: 64 columns of a row to a block, its records dealt out to GROUPS groups of 16 threads: what counts is that all are asked for at
 // once. grid (row, sequence, HD / 64)
@@ -446,7 +451,7 @@ __global__ void __launch_bounds__(16 * GROUPS) kv8_merge_kernel(const Kv8DecodeP
     cwk_pdl_launch();
     cwk_pdl_wait();
     Kv8Sum s;
-    kv8_add_records(s, Kv8Records(p, HD, b, row / p.nh, row % p.nh), column, g, GROUPS);
+    kv8_add_records(s, Kv8Records(p, HD, b, row / p.nh(), row % p.nh()), column, g, GROUPS);
     if (t == 0) { s_m[g] = s.M; s_l[g] = s.den; }
     s_o[g][t] = s.o;
     __syncthreads();
@@ -456,7 +461,7 @@ __global__ void __launch_bounds__(16 * GROUPS) kv8_merge_kernel(const Kv8DecodeP
     for (int j = 0; j < GROUPS; j++) all.M = fmaxf(all.M, s_m[j]);
 #pragma unroll
     for (int j = 0; j < GROUPS; j++) all.add(s_m[j] == -INFINITY ? 0.f : exp2f(s_m[j] - all.M), s_l[j], s_o[j][t]);
-    all.write(p.out + ((int64_t)b * p.n * p.nh + row) * HD + column);
+    all.write(p.out + ((int64_t)b * p.n * p.nh() + row) * HD + column);
 }
 
 template <int HD, int NB, bool WHOLE>
@@ -478,7 +483,7 @@ int launch(cwk_ctx *ctx, const Kv8DecodeParams &p, int type, int blocks) {
     // Records per query row; the threads that a group of 16 for every 64 columns of a row makes. Groups as long as there are records for them
     // and the SMs are not filled more than once (37 tokens of 32 heads after 300 rows, 222 blocks, 12 records a row, 1184 rows: 26.8 us with eight
     // groups a row, 15.2 with one).
-    const int64_t each = (int64_t)blocks * (GW / p.hb) / ((int64_t)p.steps.B * p.steps.groups), rows = p.n * p.nh, threads = rows * p.steps.B * (HD / 4);
+    const int64_t each = (int64_t)blocks * (GW / p.hb) / ((int64_t)p.steps.B * p.steps.groups), rows = p.n * p.nh(), threads = rows * p.steps.B * (HD / 4);
     const int64_t room = std::min<int64_t>((int64_t)ctx->sm_count * 1536 / threads, each / 2);
     if (each > 8 && room >= 4) {
         const int groups = room >= 16 ? 16 : room >= 8 ? 8 : 4;
@@ -554,7 +559,8 @@ int cwk_kv8_streams(cwk_ctx *ctx, const void *q, const cwk_kv8 &c, const int32_t
     p.q = (const uint16_t *)q; p.k = (const uint8_t *)c.k; p.v = (const uint8_t *)c.v; p.ks = c.k_scale; p.vs = c.v_scale; p.rows = c.rows;
     const Kv8Shape shape(ctx->sm_count, B, max_kv_len, n, nh, c.nkv, c.hd, max_blocks);
     const int blocks = shape.blocks;
-    p.n = n; p.nh = nh; p.nkv = c.nkv; p.group = nh / c.nkv; p.hb = shape.hb; p.per = shape.per; p.parts = shape.parts;
+    p.n = n; p.nkv = c.nkv; p.parts = shape.parts;
+    p.group = (uint8_t)(nh / c.nkv); p.hb = (uint8_t)shape.hb; p.per = (uint8_t)shape.per;
     p.lb = c.block == 32 ? 5 : c.block == 64 ? 6 : 7;
     p.scale_log2 = scale * 1.4426950408889634f;
     if (shape.groups > 0x7FFFFFFF) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_decode_kv8: too many query tokens");

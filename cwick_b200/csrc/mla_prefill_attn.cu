@@ -87,7 +87,7 @@ struct AttnParams {
     int group;          // GQA: query heads per KV head (MLA: unused)
     int64_t pos0;
     float scale_log2;
-    int spread;         // items of all heads from the longest to the shortest
+    int spread, run;    // spread: items of all heads from the longest to the shortest; run: query tiles, or (spread) heads
     int *flags;         // one word per item (share mode: per item + share): fast form sets it, exact form runs only where it is set
     int *counter;       // [3]: item counters of the fast and the exact form, number of flags raised; zero at launch
     int *err;
@@ -110,9 +110,10 @@ struct AttnItem {
 // a head whose longest items begin last is waited for, 2000 tokens of 24 heads of 128 58.7 us against 51.6.) (MLA: each of the two halves of the value columns does it.)
 __device__ __forceinline__ AttnItem attn_item(int w, const AttnParams &p, int nq) {
     AttnItem it;
-    const int qtile = nq - 1 - (p.spread ? w / p.nh : w % nq);
+    const int major = w / p.run, minor = w - major * p.run;
+    const int qtile = nq - 1 - (p.spread ? major : minor);
     it.q0 = qtile * PA_QT;
-    it.h = p.spread ? w % p.nh : w / nq;
+    it.h = p.spread ? minor : major;
     it.half = 0;
     const int64_t last_q = p.pos0 + min(it.q0 + PA_QT - 1, p.n - 1);     // keys 0 .. pos0 + (last query of the item): tiles of 64
     it.lo = 0;
@@ -1223,6 +1224,7 @@ int attn_launch(cwk_ctx *ctx, AttnParams ap, const CUtensorMap &tm_k, const CUte
         if (s != CWK_OK) return s;
         ap.shares = G; ap.records = ctx->scratch; ap.spread = 0;
     }
+    ap.run = ap.spread ? ap.nh : nq;
     const int nflags = total + (ap.shares ? G : 0);
     ap.counter = ap.flags + nflags;
     CWK_CUDA(ctx, cudaMemsetAsync(ap.flags, 0, (size_t)(nflags + 3) * sizeof(int), ctx->stream));
