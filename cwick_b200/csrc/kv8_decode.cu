@@ -28,16 +28,17 @@ struct Kv8DecodeParams {
     const uint16_t *q;                // bf16 [B][n][nh][hd]
     const uint8_t *k, *v, *ks, *vs;
     int64_t rows;                     // per slot
-    int n, nkv, parts;                // parts = ceil(n / per)
-    uint8_t group, hb, lb, per;       // hb: KV heads a block works on at once (4, 2 or 1); block = 1 << lb; per: query tokens whose heads share the MMA columns
-    float scale_log2;
     uint16_t *out;                    // bf16 [B][n][nh][hd]
     float *rec;                       // [slot][warp]: o [per * group][hd], then {m, l} [per * group]
-    __host__ __device__ int nh() const { return nkv * group; }
     GqaSteps steps;                   // groups: (nkv / hb) * parts, the parts of the same keys next to each other; keys: GK * (GW / hb)
+    int n, nkv, group, hb, lb;        // hb: KV heads a block works on at once (4, 2 or 1); block = 1 << lb
+    int per, parts;                   // query tokens whose heads share the MMA columns; parts = ceil(n / per)
+    float scale_log2;
+    __host__ __device__ int nh() const { return nkv * group; }
 };
 
-// (Parameters of more than 128 bytes come later: with eight more a step of one sequence of 4096 rows took 9.3 us instead of 8.2.)
+// (Parameters of more than 128 bytes, or of bytes, come later: with eight bytes more a step of one sequence of 4096 rows took 9.3 us instead
+// of 8.2, with heads and shifts as bytes 8.9.)
 static_assert(sizeof(Kv8DecodeParams) <= 128, "kernel parameters");
 
 __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -560,7 +561,7 @@ int cwk_kv8_streams(cwk_ctx *ctx, const void *q, const cwk_kv8 &c, const int32_t
     const Kv8Shape shape(ctx->sm_count, B, max_kv_len, n, nh, c.nkv, c.hd, max_blocks);
     const int blocks = shape.blocks;
     p.n = n; p.nkv = c.nkv; p.parts = shape.parts;
-    p.group = (uint8_t)(nh / c.nkv); p.hb = (uint8_t)shape.hb; p.per = (uint8_t)shape.per;
+    p.group = nh / c.nkv; p.hb = shape.hb; p.per = shape.per;
     p.lb = c.block == 32 ? 5 : c.block == 64 ? 6 : 7;
     p.scale_log2 = scale * 1.4426950408889634f;
     if (shape.groups > 0x7FFFFFFF) return cwk_fail(ctx, CWK_ERR_ARGUMENT, "gqa_decode_kv8: too many query tokens");
