@@ -62,6 +62,13 @@ struct Raw {
     }
     // bits of the largest magnitude; 0x7F800000 and up: there is a value that is not finite
     __device__ __forceinline__ uint32_t magnitude() const {
+        if constexpr (SRC == SRC_BF16) {                   // two at a time (a NaN wins)
+            __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&w[0]));
+#pragma unroll
+            for (int i = 1; i < W; i++) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&w[i])));
+            const uint32_t u = *reinterpret_cast<const uint32_t *>(&m);
+            return max(u & 0x7FFF0000u, (u << 16) & 0x7FFF0000u);
+        }
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < V; i++) m = max(m, __float_as_uint((*this)[i]) & 0x7FFFFFFFu);
@@ -174,6 +181,9 @@ __device__ __forceinline__ void store_words(uint8_t *dst, const uint32_t (&w)[V 
     if constexpr (V == 8) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t *>(dst) = w[0];
 }
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
 // Codes of values in units of the scale. careful: some are not finite, or larger than the largest code.
 template <int V, bool I8>
 __device__ __forceinline__ void codes_of(const float (&y)[V], bool careful, bool is_v, uint32_t (&w)[V / 4]) {
@@ -190,9 +200,27 @@ __device__ __forceinline__ void codes_of(const float (&y)[V], bool careful, bool
             uint32_t u[4];                     // plus 1.5 * 2^23: the nearest whole number (ties to even) in the low bits
 #pragma unroll
             for (int j = 0; j < 4; j++) u[j] = __float_as_uint(t[j] + 12582912.f);
-            w[i] = __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+            w[i] = low_bytes(u[0], u[1], u[2], u[3]);
         } else w[i] = kv8_encode4<I8>(t);
     }
+}
+// The same of x * f, f a power of two: the product is exact, so it goes with the addition.
+template <int V, bool I8, class X>
+__device__ __forceinline__ void store_scaled(uint8_t *dst, const X &x, float f, bool careful, bool is_v) {
+    uint32_t w[V / 4];
+    if (I8 && !careful) {
+        uint32_t u[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) u[j] = __float_as_uint(__fmaf_rn(x[j], f, 12582912.f));
+#pragma unroll
+        for (int i = 0; i < V / 4; i++) w[i] = low_bytes(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+    } else {
+        float y[V];
+#pragma unroll
+        for (int j = 0; j < V; j++) y[j] = x[j] * f;
+        codes_of<V, I8>(y, careful, is_v, w);
+    }
+    store_words<V>(dst, w);
 }
 template <int V, bool I8>
 __device__ __forceinline__ void store_codes(uint8_t *dst, const float (&y)[V], bool careful, bool is_v) {
@@ -449,10 +477,7 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
 #pragma unroll
     for (int i = 0; i < ROWS; i++, dst += ld) {
         if (i >= mine) break;
-        float y[V];
-#pragma unroll
-        for (int j = 0; j < V; j++) y[j] = x[i][j] * f;
-        store_codes<V, I8>(dst, y, careful, is_v);
+        store_scaled<V, I8>(dst, x[i], f, careful, is_v);
     }
 }
 
