@@ -13,6 +13,9 @@
 // 2^-25 of that value, 2^-16 of a bf16 step. Probabilities are f16 in [0, 2^8], three bits finer than bf16's; their sums are f32. The
 // scales are powers of two: a step's 32 keys are in one block, the key scale multiplies its scores and the value scale its product
 // on the way into the f32 accumulators, so no code's value is ever rounded or out of f16's range.
+//
+// What bounds it: a batch by HBM, 64 sequences of 4096 rows (16 heads, 4 KV heads of 256, 537 MB) 91 us = 5.9 TB/s, INT8 the same, four tokens each 108;
+// less by the start and the end of the streams, 16 sequences 32 us, one 8.3, of 32768 rows 21 (replayed).
 #include <algorithm>
 
 #include "gqa_steps.cuh"
@@ -443,7 +446,7 @@ __global__ void __launch_bounds__(256) kv8_merge_few_kernel(const Kv8DecodeParam
     s.write(p.out + ((int64_t)b * p.n * p.nh() + row) * HD + column);
 }
 // Many: 64 columns of a row to a block, its records dealt out to GROUPS groups of 16 threads: what counts is that all are asked for at
-// once. grid (row, sequence, HD / 64)
+// once (one sequence of 4096 rows has 128 records a row). grid (row, sequence, HD / 64)
 template <int HD, int GROUPS>
 __global__ void __launch_bounds__(16 * GROUPS) kv8_merge_kernel(const Kv8DecodeParams p) {
     __shared__ float s_m[GROUPS], s_l[GROUPS];

@@ -290,7 +290,8 @@ typedef struct cwk_kv8 {
 } cwk_kv8;
 
 /* Rows pos[b] .. pos[b] + count[b] - 1 of slots b = 0 .. B - 1 from k, v [B][n][nkv][hd], bf16 or (f32 != 0) f32; pos, count int32
- * [B] on the device, count NULL: n each, otherwise at most n (what is more is not read). Rows outside the slot are left out.
+ * [B] on the device, count NULL: n each, otherwise at most n (what is more is not read). Rows behind the slot's last are
+ * left out, and a slot whose position is negative gets none.
  * A block's exponent is the least e with |x| <= 448 * 2^e (E4M3; INT8: 127) for its finite new values, within [-100, 119]
  * (INT8: 121); a block that begins before pos[b] is open: rows in front of pos[b] stay what they are, e is at least the block's old one, and where
  * it grows their codes move to the new scale, rounded to nearest (E4M3: exact unless they become subnormal). code = x / 2^e to
@@ -299,8 +300,8 @@ typedef struct cwk_kv8 {
  * scale of the last block is no longer theirs. */
 CWK_API int cwk_kv8_store(cwk_ctx *ctx, const cwk_kv8 *cache, const void *k, const void *v, int f32, const int32_t *pos, const int32_t *count,
                           int B, int n);
-/* The other way: the values of rows pos[b] + j, j < count[b] (NULL: n), into k, v [B][n][nkv][hd], bf16 or (f32 != 0) f32, exactly. Rows
- * outside the slot and rows from count[b] on are left as they were. */
+/* The other way: the values of rows pos[b] + j, j < count[b] (NULL: n), into k, v [B][n][nkv][hd], bf16 or (f32 != 0) f32, exactly. What
+ * belongs to rows behind the slot's last, to rows from count[b] on and to a negative position is left as it was. */
 CWK_API int cwk_kv8_load(cwk_ctx *ctx, const cwk_kv8 *cache, const int32_t *pos, const int32_t *count, int B, int n, void *k, void *v, int f32);
 /* cwk_gqa_qk_prep for B slots at positions of their own and this cache: RMS norm with (1 + w) weights of query and key heads, rotate-half
  * RoPE on the first `rot` values (a multiple of 16), queries to bf16, keys and values into the cache as cwk_kv8_store does. qg f32

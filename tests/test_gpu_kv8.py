@@ -146,6 +146,15 @@ def test_load_gives_every_value_exactly(attn, kind, dtype, hd, nkv):
     assert np.array_equal(v[2, 0].double().cpu().numpy(), vals[1][2, 255], equal_nan=True)
 
 
+def test_load_of_a_negative_position_writes_nothing(attn):
+    c = cache_of(3, 128, 2, 128, 64, "int8")
+    want = plain_of(c)[1].values()
+    out = tuple(torch.full((3, 9, 2, 128), -7.0, device="cuda") for _ in range(2))
+    attn.kv8_load(c, i32([-4, 0, -(2 ** 31)]), 9, out=out)
+    assert (out[1][0] == -7.0).all() and (out[1][2] == -7.0).all()
+    assert np.array_equal(out[1][1].double().cpu().numpy(), want[1, :9])
+
+
 def test_offsets_beyond_32_bits(attn):
     """A cache of 2.6 GB a tensor: rows of the last slot, and of the end of the first one."""
     from cwick_b200.ops import Kv8Cache
