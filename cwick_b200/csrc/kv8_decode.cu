@@ -509,10 +509,15 @@ namespace {
 
 // The shape of a pass over `B` sequences of up to `len` rows, and what it takes.
 //
-// Whole: a block for each head group, no records, no merge and its launch. Otherwise equal shares of all steps. By a cost of each side, in us a
-// call replayed, fitted to 1 to 64 sequences of 20 to 700 rows, one and four tokens (and in shares to 580 chunks of 4 to 300 tokens after 0 to
-// 12000 rows); a launch less is worth a microsecond to whoever launches. Whole / shares, 16 heads, 4 KV heads of 256: one sequence of 20 rows
-// 4.7 / 7.8, of 100 9.4 / 7.8; 64 of 60 6.8 / 9.9, of 200 13.5 / 14.9, of 400 21.4 / 17.1; 4 tokens, 64 of 60 10.0 / 16.4.
+// Whole: a block for each head group of each sequence, no records, no merge and its launch; of one KV head, four or two, whichever gives the
+// sooner end. Otherwise equal shares of all steps. By a cost of each side, in us a call replayed, fitted to 1 to 140 sequences of 20 to 4096
+// rows, one and four tokens (and in shares to 580 chunks of 4 to 300 tokens after 0 to 12000 rows): steps one after another, or the bytes
+// at 7 TB/s (shares 6.5) where there are many blocks. The host knows the longest length only. Shares even out what is shorter, whole blocks do not:
+// so the shares count with five sixths of the rows (half ragged), and whole blocks are for lengths whose steps alone take no more than twice what
+// shares of next to nothing take (one long sequence among short ones). A launch less is worth a microsecond to whoever launches.
+// Whole / shares, 16 heads, 4 KV heads of 256: one sequence of 100 rows 4.9 / 7.4, of 600 10.6 / 7.5; 16 of 128 5.1 / 8.9, of 500 9.8 / 12.0, of 2000
+// 27 / 21; 64 of 300 12.0 / 18.8, of 1200 28.7 / 36.7 (ragged from half to that 26 / 30; one of them and 63 of 100 rows 19 / 14), of 4096 80 / 92 (73 / 71); 80 of 1200, two more blocks
+// than two for each SM, 51 / 44. Four tokens: 16 of 500 15.6 / 15.0, 64 of 1200 38 / 54 (37 / 46).
 struct Kv8Shape {
     int hb, per, parts, keys, cols, blocks;
     int64_t groups;
@@ -520,23 +525,43 @@ struct Kv8Shape {
     double us;
     Kv8Shape(int sm_count, int B, int64_t len, int n, int nh, int nkv, int hd, int max_blocks) {
         const int group = nh / nkv;
-        hb = nkv % 4 == 0 ? 4 : nkv % 2 == 0 ? 2 : 1;
         per = std::min(n, std::max(1, 16 / group));
         parts = (n + per - 1) / per;
-        keys = GK * (GW / hb);
         cols = per * group;
-        groups = (int64_t)(nkv / hb) * parts;
-        const int64_t each = (len + keys - 1) / keys, all = B * groups, steps = all * each, sms = sm_count;
-        // as many blocks as there can be steps, at most two per SM
-        blocks = (int)std::min<int64_t>(std::max<int64_t>(1, steps), max_blocks > 0 ? std::min<int64_t>(max_blocks, 2 * sms) : 2 * sms);
         const bool wide = hd == 256, two = cols > 8;
+        const int64_t sms = sm_count, slots = 2 * sms;
+        const auto deal = [&](int heads) {
+            hb = heads;
+            keys = GK * (GW / hb);
+            groups = (int64_t)(nkv / hb) * parts;
+            return (len + keys - 1) / keys;
+        };
+        double one = 1e30, alone = 0;
+        int best = 1;
+        for (int h = 4; h >= 1; h /= 2) {
+            if (nkv % h != 0) continue;
+            const int64_t each = deal(h), all = B * groups, rounds = (all + slots - 1) / slots;
+            if (all >= 1 << 30) continue;
+            const auto step = [&](int64_t blocks) {       // of a block with so many beside it
+                const double chain = (two ? (wide ? 2.05 : 1.2) : (wide ? 1.42 : 1.02)) * (blocks > sms ? 1.4 : 1.0);
+                return std::max(chain, (double)(blocks * 2 * GW * GK * hd / parts) / 7e6);
+            };
+            const double ends = (two ? (wide ? 5.7 : 4.8) : (wide ? 3.9 : 3.2)) + (h < GW ? 0.3 + 0.3 * h * cols / GW : 0.0);
+            const double x = each * ((rounds - 1) * step(slots) + step(all - (rounds - 1) * slots)) + 4.0 * (rounds - 1) + ends;
+            if (x < one) { one = x; alone = each * step(1) + ends; best = h; }
+        }
+        const int64_t each = deal(nkv % 4 == 0 ? 4 : nkv % 2 == 0 ? 2 : 1), steps = B * groups * each;
+        // as many blocks as there can be steps, at most two per SM
+        blocks = (int)std::min<int64_t>(std::max<int64_t>(1, steps), max_blocks > 0 ? std::min<int64_t>(max_blocks, slots) : slots);
         const double turns = (double)((steps + blocks - 1) / blocks), records = (double)blocks * GW * cols * hd * 4e-6;
-        const double shares = (wide ? 6.8 : 6.0) + turns * (two ? (wide ? 3.1 : 1.85) : (wide ? 0.94 : 0.82)) + 0.65 * records;
-        const double one = (double)(((all + 2 * sms - 1) / (2 * sms)) * each) * (two ? (wide ? 2.1 : 1.22) : (wide ? 1.35 : 1.03)) * (all > sms ? 1.3 : 1.0) +
-                           (two ? (wide ? 5.7 : 4.8) : (wide ? 3.9 : 3.2)) + (hb < GW ? 0.7 + 0.3 * hb * cols / GW : 0.0);
-        whole = max_blocks == 0 && all < (1 << 30) && one <= shares + 1.0;
-        us = whole ? one : shares;
-        if (whole) blocks = (int)all;
+        const double stream = std::max(turns * (two ? (wide ? 3.1 : 1.85) : (wide ? 0.94 : 0.82)), (double)B * len * nkv * hd * 2 / 6.5e6);
+        const double shares = (wide ? 6.8 : 6.0) + (B > 1 ? 1.5 : 0.0) + 0.65 * records;
+        whole = max_blocks == 0 && one <= shares + stream * (B > 1 ? 5.0 / 6 : 1.0) + 1.0 && (B == 1 || alone <= 2 * shares);
+        if (whole) {
+            deal(best);
+            blocks = (int)(B * groups);
+        }
+        us = whole ? one : shares + stream;
     }
 };
 
