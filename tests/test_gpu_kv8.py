@@ -289,6 +289,18 @@ def test_decode_of_ragged_batches(attn, kind, hd, nh, nkv, lens):
     check_decode(attn, c, k, v, q, lens)
 
 
+@pytest.mark.parametrize("n,hd,kind", [(1, 256, "e4m3"), (1, 128, "int8"), (4, 256, "int8")])
+@pytest.mark.parametrize("B,most,nh,nkv", [(5, 130, 16, 4), (40, 300, 16, 4), (90, 300, 16, 4), (100, 60, 8, 2), (40, 300, 32, 8), (160, 200, 16, 4)])
+def test_decode_of_many_short_sequences(attn, n, hd, kind, B, most, nh, nkv):
+    """Blocks of one, two and four KV heads that have a sequence to themselves, one round of them and more."""
+    rows = -(-most // 32) * 32
+    c, k, v = filled(attn, B, rows, nkv, hd, 32, kind, seed=B + n)
+    lens = torch.randint(0, most + 1, (B,), generator=torch.Generator().manual_seed(B)).tolist()
+    lens[:5] = [most, 0, 1, 33, 32]
+    q = torch.randn(B, n, nh, hd, device="cuda", generator=gen(B)).to(torch.bfloat16)
+    check_decode(attn, c, k, v, q, lens)
+
+
 @pytest.mark.parametrize("block", [32, 128])
 @pytest.mark.parametrize("n,nh,nkv", [(2, 16, 4), (4, 16, 4), (5, 16, 4), (3, 6, 2), (2, 24, 3), (17, 8, 8), (3, 16, 1)])
 @pytest.mark.parametrize("hd,lens", [(256, [700, 0, 1, 33]), (128, [2, 1031])])
