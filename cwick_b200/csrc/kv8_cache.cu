@@ -394,7 +394,9 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
             for (int i = 0; i < ROWS; i++) {
                 if (i >= mine) break;
                 const float r = rsqrtf(warp_sum(squares<V, float>(x[i])) * (1.f / HD) + p.eps);
-                unsure |= !(r > 1e-15f && r < 1e30f);      // (where squares leave the range or are too small for it)
+                // (where squares leave float's range, or are so small that they have few bits: with r < 1e17 the sum of 128 squares or more is
+                // above 2^-106, and what each loses below 2^-149 is nothing beside it)
+                unsure |= !(r > 1e-15f && r < 1e17f);
                 norm_rotate<V, float>(x[i], r, w1, p.rot, lane, csf + i * pairs, y[i]);
 #pragma unroll
                 for (int j = 0; j < V; j++) amax = max(amax, __float_as_uint(y[i][j]) & 0x7FFFFFFFu);

@@ -243,6 +243,28 @@ def test_prep_of_extreme_rows(attn, kind, eps):
     same(c, want)
 
 
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("eps", [0.0, float(np.float32(1e-40)), float(np.float32(1e-32))])
+@pytest.mark.parametrize("hd,alone", [(256, True), (128, True), (256, False)])
+def test_prep_of_keys_whose_squares_are_subnormal(attn, kind, eps, hd, alone):
+    """Without an epsilon that outweighs them, rows down to 1e-23 have a sum of squares in float that is not zero and has few bits: a block for
+    each size, in which one row is that small (no other row casts doubt on the block) or all are."""
+    sizes = [1e-15, 1e-16, 1e-17, 1e-18, 1e-19, 1e-20, 1e-21, 1e-22, 3e-23, 1e-23]
+    nh, nkv, rot, block, theta, n = 1, 2, 64, 32, 1e4, 32 * len(sizes)
+    g = gen(11)
+    qg = torch.randn(1, n, nh, 2 * hd, device="cuda", generator=g)
+    k, v = (torch.randn(1, n, nkv, hd, device="cuda", generator=g) for _ in range(2))
+    for i, size in enumerate(sizes):
+        k[:, 32 * i + 13:32 * i + 14 if alone else 32 * i + 32] *= size
+    qn, kn = (0.1 * torch.randn(hd, device="cuda", generator=g) for _ in range(2))
+    c = cache_of(1, n, nkv, hd, block, kind)
+    want = plain_of(c)
+    attn.gqa_qk_prep_kv8(c, qg, k, v, qn, kn, eps, rot, theta, i32([0]))
+    want[0].store(plain.norm_rotate(k[0].double().cpu().numpy(), kn.cpu().numpy(), eps, rot, theta, np.arange(n))[None], [0], [n])
+    want[1].store(v.double().cpu().numpy(), [0], [n])
+    same(c, want)
+
+
 # ---- decode -------------------------------------------------------------------------------------------------------------------
 
 def filled(attn, slots, rows, nkv, hd, block, kind, seed, climb=False):
