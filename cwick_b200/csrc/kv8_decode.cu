@@ -284,9 +284,11 @@ __global__ void __launch_bounds__(32 * GW, 2) kv8_decode_kernel(const Kv8DecodeP
                 for (int x = 0; x < 2; x++)
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) big[x] = fmaxf(big[x], __shfl_xor_sync(0xffffffffu, big[x], o));
-                if (fresh) {                              // (a row that sees none of these keys sees none behind them: any exponent will do)
-                    m[nb][0] = big[0] == -INFINITY ? 0.f : big[0];
-                    m[nb][1] = big[1] == -INFINITY ? 0.f : big[1];
+                if (fresh) {
+                    // A row that sees none of these keys sees none behind them: any exponent will do. And where all that it sees is NaN: its sum
+                    // is NaN, which the merge keeps, but a NaN for exponent would lose against any other, or -infinity.
+                    m[nb][0] = big[0] > -INFINITY ? big[0] : 0.f;
+                    m[nb][1] = big[1] > -INFINITY ? big[1] : 0.f;
                 } else {
                     float f[2];
 #pragma unroll

@@ -373,6 +373,24 @@ def test_decode_of_nan_rows(attn):
     assert bool(got[0, 1:].isnan().all())
 
 
+@pytest.mark.parametrize("n", [1, 4])
+@pytest.mark.parametrize("lens,n_splits", [([4096], 0), ([4096], 5), ([4096, 700], 0), ([90] * 40, 0), ([300] * 90, 0), ([2500] + [40] * 70, 0)])
+def test_decode_of_sequences_of_nan_rows(attn, n, lens, n_splits):
+    """Sequences of NaN keys alone, and of 128 at the front: what warps leave of them has no score to be the reference exponent, and every query
+    row shows it, however the rows are dealt out and joined. A sequence beside them does not."""
+    nh, nkv, hd = 16, 4, 256
+    rows = -(-max(lens) // 64) * 64
+    for bad in (rows, 128):
+        c = cache_of(len(lens), rows, nkv, hd, 64, "e4m3")
+        k, v = (rows_of(i, (len(lens), rows, nkv, hd), torch.bfloat16) for i in range(2))
+        k[0, :bad] = float("nan")
+        attn.kv8_store(c, k, v, i32([0] * len(lens)))
+        q = torch.randn(len(lens), n, nh, hd, device="cuda", generator=gen(1)).to(torch.bfloat16)
+        got = attn.gqa_decode_kv8(q, c, i32(lens), max_kv_len=max(lens), n_splits=n_splits)
+        assert bool(got[0].isnan().all())
+        assert bool(got[1:].isfinite().all())
+
+
 def test_decode_gives_the_same_bits_again(attn):
     c, k, v = filled(attn, 3, 1024, 4, 256, 64, "e4m3", seed=8)
     q = torch.randn(3, 16, 256, device="cuda", generator=gen(2)).to(torch.bfloat16)
@@ -399,6 +417,27 @@ def test_prefill_against_64_bits(attn, kind, n, pos, nh, nkv, hd):
     want, tol = plain.attend(Q.double(), k[1, :T], v[1, :T], pos + 1 + torch.arange(n, device="cuda"), hd ** -0.5, BF16)
     off = (got.double() - want).abs()
     assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.parametrize("n,pos,nh,nkv,hd", [(5, 1000, 16, 4, 256), (300, 0, 16, 4, 256), (257, 3000, 8, 2, 256), (300, 0, 24, 3, 128), (150, 3000, 16, 2, 128)])
+@pytest.mark.parametrize("bad", ["front", "last"])
+def test_prefill_of_nan_rows(attn, n, pos, nh, nkv, hd, bad):
+    """NaN keys reach the queries that see them and no other, by streams and by tensor cores, in shares or not."""
+    T = pos + n
+    rows = -(-T // 64) * 64
+    c = cache_of(1, rows, nkv, hd, 64, "e4m3")
+    k, v = (rows_of(i, (1, rows, nkv, hd), torch.bfloat16) for i in range(2))
+    if bad == "front":
+        k[0, :128] = float("nan")
+    else:
+        k[0, T - 3] = float("nan")
+    attn.kv8_store(c, k, v, i32([0]))
+    got = attn.gqa_prefill_kv8(torch.randn(n, nh, hd, device="cuda", generator=gen(n)).to(torch.bfloat16), c, pos)
+    attn.ctx.sync()
+    if bad == "front":
+        assert bool(got.isnan().all())
+    else:
+        assert bool(got[:n - 3].isfinite().all()) and bool(got[n - 3:].isnan().all())
 
 
 # ---- together -------------------------------------------------------------------------------------------------------------------
