@@ -269,6 +269,42 @@ __device__ __forceinline__ void rescale(uint8_t *codes, int64_t ld, int lead, in
     }
 }
 
+// A reciprocal root in float of squares that leave float's range, or are so small that they have few bits: below 1e17 the sum of 128 squares
+// or more is above 2^-106, and what each loses below 2^-149 is nothing beside it.
+__device__ __forceinline__ bool out_of_range(float rstd) { return !(rstd > 1e-15f && rstd < 1e17f); }
+template <int V>
+__device__ __forceinline__ void store_query(uint16_t *dst, const float (&y)[V]) {
+    uint32_t o[V / 2];
+#pragma unroll
+    for (int k = 0; k < V / 2; k++) o[k] = pack_bf16x2(y[2 * k], y[2 * k + 1]);
+    if constexpr (V == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    else *reinterpret_cast<uint2 *>(dst) = make_uint2(o[0], o[1]);
+}
+// Those of query heads h0 .. h0 + heads - 1 of a token again, multiplied by a power of two first, and epsilon by its square: large rows (root of the
+// mean 2^49 and up) come below 2^48, small ones are at most 2^44, the least subnormal 2^-49. (Not inlined: to 7 x 300 rows that
+// have no use for it, 19.6 us, it adds 0.9 in line and so 0.5.)
+template <int V>
+__device__ __noinline__ void query_rows_out_of_range(const Kv8PrepParams &p, int64_t t, int h0, int heads, int lane, const float2 *csf) {
+    constexpr int HD = 32 * V;
+    Raw<V, SRC_F32> w;
+    w.load(p.q_norm, 0, lane);
+    float w1[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) w1[i] = 1.f + w[i];
+#pragma unroll 1
+    for (int i = 0; i < heads; i++) {
+        Raw<V, SRC_F32> x;
+        x.load(p.qg, (t * p.nh + h0 + i) * 2, lane);
+        const float sum = warp_sum(squares<V, float>(x)), unit = sum > 1.f ? 0x1p-80f : 0x1p100f;
+        if (!out_of_range(rsqrtf(sum * (1.f / HD) + p.eps))) continue;
+        float z[V], y[V];
+#pragma unroll
+        for (int k = 0; k < V; k++) z[k] = x[k] * unit;
+        norm_rotate<V, float>(z, rsqrtf(warp_sum(squares<V, float>(z)) * (1.f / HD) + p.eps * unit * unit), w1, p.rot, lane, csf, y);
+        store_query<V>(p.q_out + (t * p.nh + h0 + i) * HD + lane * V, y);
+    }
+}
+
 // V: values of a row per lane (head dim / 32); ROWS: rows of a warp. PREP: f32 rows, keys normed and rotated; blocks from p.tasks on have
 // query rows.
 template <int V, int SRC, bool I8, class PARAMS, int ROWS>
@@ -299,18 +335,18 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
         float w1[V];
 #pragma unroll
         for (int i = 0; i < V; i++) w1[i] = 1.f + w[i];
+        float least = 1.f, most = 1.f;                     // of the reciprocal roots
 #pragma unroll
         for (int i = 0; i < KQ_HEADS; i++) {
             if (i >= heads) break;
+            const float r = rsqrtf(warp_sum(squares<V, float>(x[i])) * (1.f / HD) + p.eps);
+            least = fminf(least, r);
+            most = fmaxf(most, r);
             float y[V];
-            norm_rotate<V, float>(x[i], rsqrtf(warp_sum(squares<V, float>(x[i])) * (1.f / HD) + p.eps), w1, p.rot, lane, csf, y);
-            uint32_t o[V / 2];
-#pragma unroll
-            for (int k = 0; k < V / 2; k++) o[k] = pack_bf16x2(y[2 * k], y[2 * k + 1]);
-            uint16_t *dst = p.q_out + (t * p.nh + h0 + i) * HD + lane * V;
-            if constexpr (V == 8) *reinterpret_cast<uint4 *>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-            else *reinterpret_cast<uint2 *>(dst) = make_uint2(o[0], o[1]);
+            norm_rotate<V, float>(x[i], r, w1, p.rot, lane, csf, y);
+            store_query<V>(p.q_out + (t * p.nh + h0 + i) * HD + lane * V, y);
         }
+        if (least <= 1e-15f || most >= 1e17f) query_rows_out_of_range<V>(p, t, h0, heads, lane, csf);
         return;
     }
     uint32_t id = blockIdx.x;
@@ -394,9 +430,7 @@ __global__ void __launch_bounds__(512, SRC == SRC_BF16 ? 2 : 1) kv8_write_kernel
             for (int i = 0; i < ROWS; i++) {
                 if (i >= mine) break;
                 const float r = rsqrtf(warp_sum(squares<V, float>(x[i])) * (1.f / HD) + p.eps);
-                // (where squares leave float's range, or are so small that they have few bits: with r < 1e17 the sum of 128 squares or more is
-                // above 2^-106, and what each loses below 2^-149 is nothing beside it)
-                unsure |= !(r > 1e-15f && r < 1e17f);
+                unsure |= out_of_range(r);
                 norm_rotate<V, float>(x[i], r, w1, p.rot, lane, csf + i * pairs, y[i]);
 #pragma unroll
                 for (int j = 0; j < V; j++) amax = max(amax, __float_as_uint(y[i][j]) & 0x7FFFFFFFu);

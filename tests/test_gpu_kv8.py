@@ -265,6 +265,25 @@ def test_prep_of_keys_whose_squares_are_subnormal(attn, kind, eps, hd, alone):
     same(c, want)
 
 
+@pytest.mark.parametrize("eps", [0.0, float(np.float32(1e-40)), 1e-6])
+@pytest.mark.parametrize("hd,nh,n", [(256, 3, 90), (128, 10, 300)])
+def test_prep_of_query_rows_of_any_size(attn, eps, hd, nh, n):
+    """Query rows whose squares leave float's range at either end, or have few bits there, beside ordinary heads of the same token."""
+    sizes = [1.0, 1e-10, 1e-15, 1e-17, 1e-18, 1e-19, 1e-20, 1e-21, 1e-22, 3e-23, 1e-30, 1e-37, 1e-42, 1e12, 1e15, 1e17, 1e18, 1e19, 1e25, 1e33, 5e37]
+    nkv, rot, theta, pos = 1, 64, 1e4, 77
+    g = gen(n)
+    size = torch.tensor(sizes, device="cuda")[torch.arange(n * nh, device="cuda") % len(sizes)].view(n, nh, 1)
+    qg = torch.randn(1, n, nh, 2 * hd, device="cuda", generator=g) * size
+    k, v = (torch.randn(1, n, nkv, hd, device="cuda", generator=g) for _ in range(2))
+    qn, kn = (0.1 * torch.randn(hd, device="cuda", generator=g) for _ in range(2))
+    c = cache_of(1, 512, nkv, hd, 64, "e4m3")
+    got = attn.gqa_qk_prep_kv8(c, qg, k, v, qn, kn, eps, rot, theta, i32([pos]))[0].double().cpu().numpy()
+    want = plain.norm_rotate(qg[0, ..., :hd].double().cpu().numpy(), qn.cpu().numpy(), float(np.float32(eps)), rot, theta, pos + np.arange(n))
+    # bf16's half step (of its least normal number below that); f32 norm and rotation as in test_prep_against_64_bits
+    size = np.abs(want).max(-1, keepdims=True)
+    assert np.all(np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -20 * size + 2.0 ** -134)
+
+
 # ---- decode -------------------------------------------------------------------------------------------------------------------
 
 def filled(attn, slots, rows, nkv, hd, block, kind, seed, climb=False):
