@@ -24,12 +24,19 @@ _I32 = torch.int32
 _ROWS = {torch.bfloat16: 0, torch.float32: 1}
 
 
-def _i32(t, B):
-    """The address of an int32 [B] cuda tensor, or None."""
+# The calls over a Kv8Cache: every tensor is on the context's GPU (get_device() of one on the host is -1).
+
+def _i32(t, B, device):
+    """The address of an int32 [B] tensor, or None."""
     if t is None:
         return None
-    assert t.dtype is _I32 and t.is_cuda and t.is_contiguous() and t.dim() == 1 and t.numel() == B
+    assert t.dtype is _I32 and t.get_device() == device and t.is_contiguous() and t.dim() == 1 and t.numel() == B
     return t.data_ptr()
+
+
+def _bf16_on(t, device):
+    assert t.dtype is torch.bfloat16 and t.get_device() == device and t.is_contiguous()
+    return t
 
 
 def _kv8_rows(cache, device, k, v):
@@ -37,7 +44,7 @@ def _kv8_rows(cache, device, k, v):
     shape, dtype = k.shape, k.dtype
     B, n, nkv, hd = shape
     assert v.shape == shape and nkv == cache.nkv and hd == cache.hd and v.dtype is dtype and dtype in _ROWS
-    assert k.is_contiguous() and v.is_contiguous() and k.is_cuda and v.is_cuda and cache.device == device
+    assert k.is_contiguous() and v.is_contiguous() and k.get_device() == device == v.get_device() and cache.device == device
     return B, n, _ROWS[dtype]
 
 
@@ -221,7 +228,7 @@ class Attn:
     def kv8_store(self, cache, k, v, pos, count=None):
         """Rows pos[b] .. of slot b from k, v [B][n][nkv][hd] (bf16 or f32); pos, count int32 [B] cuda (count None: n rows each)."""
         B, n, f32 = _kv8_rows(cache, self.device, k, v)
-        st = self._kv8_store(self.ctx.address, cache.address, k.data_ptr(), v.data_ptr(), f32, _i32(pos, B), _i32(count, B), B, n)
+        st = self._kv8_store(self.ctx.address, cache.address, k.data_ptr(), v.data_ptr(), f32, _i32(pos, B, self.device), _i32(count, B, self.device), B, n)
         if st:
             self.ctx.check(st)
 
@@ -232,7 +239,7 @@ class Attn:
         k, v = out
         B, rows, f32 = _kv8_rows(cache, self.device, k, v)
         assert rows == n
-        st = self._kv8_load(self.ctx.address, cache.address, _i32(pos, B), _i32(count, B), B, n, k.data_ptr(), v.data_ptr(), f32)
+        st = self._kv8_load(self.ctx.address, cache.address, _i32(pos, B, self.device), _i32(count, B, self.device), B, n, k.data_ptr(), v.data_ptr(), f32)
         if st:
             self.ctx.check(st)
         return k, v
@@ -244,19 +251,19 @@ class Attn:
         nh = qg.shape[2]
         assert f32 and qg.shape == (B, n, nh, 2 * cache.hd) and q_norm.numel() == k_norm.numel() == cache.hd
         for t in (qg, q_norm, k_norm):
-            assert t.dtype is torch.float32 and t.is_contiguous() and t.is_cuda
+            assert t.dtype is torch.float32 and t.is_contiguous() and t.get_device() == self.device
         if q_out is None:
             q_out = torch.empty(B, n, nh, cache.hd, dtype=torch.bfloat16, device=qg.device)
-        assert _bf16(q_out).shape == (B, n, nh, cache.hd)
+        assert _bf16_on(q_out, self.device).shape == (B, n, nh, cache.hd)
         st = self._gqa_qk_prep_kv8(self.ctx.address, qg.data_ptr(), k.data_ptr(), v.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(), eps, rot,
-                                   theta, _i32(pos, B), _i32(count, B), B, n, nh, q_out.data_ptr(), cache.address)
+                                   theta, _i32(pos, B, self.device), _i32(count, B, self.device), B, n, nh, q_out.data_ptr(), cache.address)
         if st:
             self.ctx.check(st)
         return q_out
 
     def gqa_decode_kv8(self, q, cache, kv_len, scale=None, max_kv_len=None, n_splits=0, out=None):
         """q bf16 [B][nh][hd], or [B][n][nh][hd] for n query tokens per sequence; kv_len int32 [B], those tokens' rows included."""
-        _bf16(q)
+        _bf16_on(q, self.device)
         if q.dim() == 4:
             B, n, nh, hd = q.shape
         else:
@@ -269,15 +276,15 @@ class Attn:
         if out is None:
             out = torch.empty_like(q)
         else:
-            assert _bf16(out).shape == q.shape
-        st = self._gqa_decode_kv8(self.ctx.address, q.data_ptr(), cache.address, _i32(kv_len, B), max_kv_len, B, n, nh, scale, out.data_ptr(), n_splits)
+            assert _bf16_on(out, self.device).shape == q.shape
+        st = self._gqa_decode_kv8(self.ctx.address, q.data_ptr(), cache.address, _i32(kv_len, B, self.device), max_kv_len, B, n, nh, scale, out.data_ptr(), n_splits)
         if st:
             self.ctx.check(st)
         return out
 
     def gqa_prefill_kv8(self, Q, cache, pos, slot=0, scale=None):
         """Q bf16 [n][nh][hd] at positions pos .. of a slot, whose rows up to pos + n are in the cache."""
-        _bf16(Q)
+        _bf16_on(Q, self.device)
         n, nh, hd = Q.shape
         assert hd == cache.hd and cache.device == self.device
         out = torch.empty_like(Q)

@@ -76,3 +76,62 @@ def test_the_plain_store_row_by_row_and_at_once(kind):
     unit = np.ldexp(1.0, one.scale.astype(int) - 127).repeat(32, 1)[..., None]
     assert np.all(np.abs(one.values() - all_.values()) <= (unit if kind == "int8" else unit * 2.0 ** -9))
     assert np.all(np.abs(all_.values()[:, :40] - x) <= (0.5 * unit[:, :40] if kind == "int8" else np.maximum(2.0 ** -4 * np.abs(x), 2.0 ** -10 * unit[:, :40])))
+
+
+class Elsewhere:
+    """Looks like a contiguous tensor of a GPU."""
+    is_cuda = True
+
+    def __init__(self, shape, dtype, device=0):
+        self.shape, self.dtype, self.index = torch.Size(shape), dtype, device
+
+    def get_device(self):
+        return self.index
+
+    def is_contiguous(self):
+        return True
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return self.shape.numel()
+
+    def data_ptr(self):
+        return 4096
+
+
+@pytest.mark.parametrize("what", ["kv8_store", "kv8_load", "gqa_qk_prep_kv8", "gqa_decode_kv8", "gqa_prefill_kv8"])
+def test_tensors_of_another_gpu_are_refused(what, monkeypatch):
+    """Every tensor of a call, one at a time on another GPU than the context's: refused before the address goes anywhere."""
+    from types import SimpleNamespace
+
+    from cwick_b200 import ops
+    monkeypatch.setattr(torch, "empty_like", lambda t: t)
+    B, n, nh, nkv, hd = 2, 3, 4, 2, 128
+    f32, bf16, int32 = torch.float32, torch.bfloat16, torch.int32
+    rows, row = (B, n, nkv, hd), ((B,), int32)
+    cache = SimpleNamespace(nkv=nkv, hd=hd, device=0, address=4096)
+    calls_made = []
+    attn = object.__new__(ops.Attn)
+    attn.device, attn.ctx = 0, SimpleNamespace(address=4096)
+    setattr(attn, "_" + what, lambda *a: calls_made.append(a) or 0)
+    tensors, call = {
+        "kv8_store": ([(rows, bf16), (rows, bf16), row, row], lambda k, v, pos, count: attn.kv8_store(cache, k, v, pos, count)),
+        "kv8_load": ([row, row, (rows, f32), (rows, f32)], lambda pos, count, k, v: attn.kv8_load(cache, pos, n, count, out=(k, v))),
+        "gqa_qk_prep_kv8": ([((B, n, nh, 2 * hd), f32), (rows, f32), (rows, f32), ((hd,), f32), ((hd,), f32), row, row, ((B, n, nh, hd), bf16)],
+                            lambda qg, k, v, qn, kn, pos, count, out: attn.gqa_qk_prep_kv8(cache, qg, k, v, qn, kn, 1e-6, 64, 1e4, pos, count, out)),
+        "gqa_decode_kv8": ([((B, n, nh, hd), bf16), row, ((B, n, nh, hd), bf16)],
+                           lambda q, lens, out: attn.gqa_decode_kv8(q, cache, lens, max_kv_len=64, out=out)),
+        "gqa_prefill_kv8": ([((n, nh, hd), bf16)], lambda Q: attn.gqa_prefill_kv8(Q, cache, 0)),
+    }[what]
+    call(*(Elsewhere(*t) for t in tensors))
+    assert len(calls_made) == 1
+    for away in range(len(tensors)):
+        for device in (1, -1):
+            with pytest.raises(AssertionError):
+                call(*(Elsewhere(*t, device if i == away else 0) for i, t in enumerate(tensors)))
+    cache.device = 1
+    with pytest.raises(AssertionError):
+        call(*(Elsewhere(*t) for t in tensors))
+    assert len(calls_made) == 1
