@@ -97,6 +97,13 @@ public:
         *granted = bytes;
         return cudaSuccess;
     }
+    // `want` bytes, or at least `least` where there is no memory for that.
+    cudaError_t alloc(int device, size_t want, size_t least, void **p, size_t *granted) {
+        const cudaError_t e = alloc(device, want, p, granted);
+        if (e != cudaErrorMemoryAllocation || want <= least) return e;
+        (void)cudaGetLastError();
+        return alloc(device, least, p, granted);
+    }
     cudaError_t free(int device, void *p, size_t bytes, bool idle) {
         if (!p) return cudaSuccess;
         if (idle) {

@@ -64,6 +64,8 @@ int cwk_check_cuda(cwk_ctx *ctx, cudaError_t e, const char *what);
 int cwk_reserve_scratch(cwk_ctx *ctx, size_t bytes);
 int cwk_reserve_stage(cwk_ctx *ctx, size_t dev_bytes, size_t pin_bytes);
 int cwk_reserve_work(cwk_ctx *ctx, size_t bytes);
+// The same for what grows from call to call, up to `most`: where the buffer is too small, twice what is needed.
+int cwk_reserve_work_growing(cwk_ctx *ctx, size_t bytes, size_t most);
 // After a stream synchronise: turn a kernel-side give-up code into CWK_ERR_STATE.
 int cwk_check_device_error(cwk_ctx *ctx);
 // Allocate the error word on first use: pinned, mapped host memory, so the host reads it without a copy.

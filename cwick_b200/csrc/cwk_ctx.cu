@@ -1,4 +1,5 @@
 // cwk_ctx.cu -- context lifecycle, error text, scratch and staging buffers.
+#include <algorithm>
 #include <cstdarg>
 
 #include "cwk_common.cuh"
@@ -6,7 +7,7 @@
 namespace {
 CwkBufferPool g_pool;
 
-// At least `bytes` in a buffer of the context; one that is too small makes room for one of `want`.
+// At least `bytes` in a buffer of the context; one that is too small makes room for one of `want`, or of `bytes` where there is no memory for that.
 int reserve(cwk_ctx *ctx, void **p, size_t *have, size_t bytes, size_t want) {
     ctx->use.use(ctx->stream);
     if (bytes <= *have) return CWK_OK;
@@ -18,7 +19,7 @@ int reserve(cwk_ctx *ctx, void **p, size_t *have, size_t bytes, size_t want) {
         *have = 0;
         CWK_CUDA(ctx, g_pool.free(ctx->device, old, n, ctx->use.known()));
     }
-    CWK_CUDA(ctx, g_pool.alloc(ctx->device, want, p, have));
+    CWK_CUDA(ctx, g_pool.alloc(ctx->device, want, bytes, p, have));
     return CWK_OK;
 }
 }  // namespace
@@ -41,6 +42,9 @@ int cwk_check_cuda(cwk_ctx *ctx, cudaError_t e, const char *what) {
 
 int cwk_reserve_scratch(cwk_ctx *ctx, size_t bytes) { return reserve(ctx, (void **)&ctx->scratch, &ctx->scratch_bytes, bytes, bytes + (bytes >> 2)); }
 int cwk_reserve_work(cwk_ctx *ctx, size_t bytes) { return reserve(ctx, &ctx->work, &ctx->work_bytes, bytes, bytes); }
+int cwk_reserve_work_growing(cwk_ctx *ctx, size_t bytes, size_t most) {
+    return reserve(ctx, &ctx->work, &ctx->work_bytes, bytes, std::max(bytes, std::min(2 * bytes, most)));
+}
 
 int cwk_reserve_stage(cwk_ctx *ctx, size_t dev_bytes, size_t pin_bytes) {
     if (dev_bytes > ctx->stage_dev_bytes) {

@@ -650,9 +650,11 @@ int cwk_gqa_prefill_kv8(cwk_ctx *ctx, const void *Q, const cwk_kv8 *c, int slot,
     at.k = (uint8_t *)c->k + slot * c->rows * row; at.v = (uint8_t *)c->v + slot * c->rows * row;
     at.k_scale = c->k_scale + slot * (c->rows / c->block) * c->nkv; at.v_scale = c->v_scale + slot * (c->rows / c->block) * c->nkv;
     if (kv8_streams_sooner(ctx->sm_count, pos, n, nh, c->nkv, c->hd)) return cwk_kv8_streams(ctx, Q, at, nullptr, (int)T, 1, n, nh, scale, out, 0);
-    // the slot's rows widened, exactly, behind the flags that the bf16 kernel keeps at the start of the workspace (a word per item and SM)
+    // The slot's rows widened, exactly, behind the flags that the bf16 kernel keeps at the start of the workspace (a word per item and SM).
+    // It grows by doubling, up to all of the slot's rows: a prompt's chunks ask for a little more every time (40 chunks of 512 in a
+    // context that has no workspace yet 182 ms with a buffer of its own size for each, 5 to 8).
     const size_t flags = ((((size_t)((n + 127) / 128) * nh + ctx->sm_count + 3) * sizeof(int)) + 255) & ~(size_t)255, half = (size_t)T * row * 2;
-    s = cwk_reserve_work(ctx, flags + 2 * half);
+    s = cwk_reserve_work_growing(ctx, flags + 2 * half, flags + (size_t)c->rows * row * 4);
     if (s != CWK_OK) return s;
     uint8_t *wk = (uint8_t *)ctx->work + flags;
     s = cwk_kv8_widen(ctx, at, 0, T, wk, wk + half);

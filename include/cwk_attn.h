@@ -316,7 +316,8 @@ CWK_API int cwk_gqa_qk_prep_kv8(cwk_ctx *ctx, const float *qg, const float *k, c
 CWK_API int cwk_gqa_decode_kv8(cwk_ctx *ctx, const void *q, const cwk_kv8 *cache, const int32_t *kv_len, int max_kv_len, int B, int n, int nh,
                                float scale, void *out, int n_splits);
 /* cwk_gqa_prefill over this cache: queries at positions pos .. pos + n - 1 of one slot against its first pos + n rows.
- * Q, out bf16 [n][nh][hd]. Workspace inside the context: 4 bytes per cached value. */
+ * Q, out bf16 [n][nh][hd]. Workspace inside the context: the pos + n rows in bf16 (2 bytes per key and per value), grown by doubling up to
+ * the slot's rows. */
 CWK_API int cwk_gqa_prefill_kv8(cwk_ctx *ctx, const void *Q, const cwk_kv8 *cache, int slot, int64_t pos, int n, int nh, float scale, void *out);
 
 /* ---- FP8 block-scaled projection -------------------------------------------

@@ -459,6 +459,26 @@ def test_prefill_of_nan_rows(attn, n, pos, nh, nkv, hd, bad):
         assert bool(got[:n - 3].isfinite().all()) and bool(got[n - 3:].isnan().all())
 
 
+def test_a_growing_prompts_workspace_grows_by_doubling(attn):
+    """A prompt in chunks from position 0 on, on the tensor cores: the context's workspace is taken anew a few times, not for every chunk, and ends
+    at what the slot needs."""
+    from cwick_b200.ops import Attn
+    nh, nkv, hd, n, chunks = 16, 4, 256, 512, 40
+    c, _, _ = filled(attn, 1, n * chunks, nkv, hd, 64, "e4m3", seed=3)
+    Q = torch.randn(n, nh, hd, device="cuda", generator=gen(1)).to(torch.bfloat16)
+    torch.cuda.synchronize()
+    other = Attn(0)
+    free = []
+    for i in range(chunks):
+        before = other.ctx.launches
+        other.gqa_prefill_kv8(Q, c, i * n)
+        other.ctx.sync()
+        assert other.ctx.launches - before >= 3, "not on the tensor cores"
+        free.append(torch.cuda.mem_get_info()[0])
+    # the first of 4 MB, doublings to the slot's 84; and the records of chunks dealt out in shares, a buffer of one size
+    assert len(set(free)) <= 7, free
+
+
 # ---- together -------------------------------------------------------------------------------------------------------------------
 
 def test_a_prompt_and_the_tokens_behind_it(attn):
