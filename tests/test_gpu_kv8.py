@@ -419,6 +419,19 @@ def test_decode_gives_the_same_bits_again(attn):
         assert torch.equal(attn.gqa_decode_kv8(q, c, lens), first)
 
 
+@pytest.mark.parametrize("B,length,n,nh,nkv,hd,launches", [(1, 100, 1, 16, 4, 256, 1), (1, 4000, 1, 16, 4, 256, 2), (16, 128, 1, 16, 4, 256, 1), (64, 4000, 1, 16, 4, 256, 2),
+                                                           (64, 1200, 4, 16, 4, 256, 1), (2, 3000, 4, 16, 2, 128, 2)])
+def test_decode_takes_the_form_it_is_tested_in(attn, B, length, n, nh, nkv, hd, launches):
+    """Whole blocks are one launch, shares and their merge two: lengths far from where the cost changes sides."""
+    rows = -(-length // 64) * 64
+    c, k, v = filled(attn, B, rows, nkv, hd, 64, "int8", seed=B)
+    q = torch.randn(B, n, nh, hd, device="cuda", generator=gen(B)).to(torch.bfloat16)
+    lens = [length - b for b in range(B)]
+    before = attn.ctx.launches
+    check_decode(attn, c, k, v, q, lens)
+    assert attn.ctx.launches - before == launches
+
+
 # ---- prompt chunks --------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kind", ["e4m3", "int8"])
@@ -457,6 +470,56 @@ def test_prefill_of_nan_rows(attn, n, pos, nh, nkv, hd, bad):
         assert bool(got.isnan().all())
     else:
         assert bool(got[:n - 3].isfinite().all()) and bool(got[n - 3:].isnan().all())
+
+
+@pytest.mark.parametrize("climb", [False, True])
+@pytest.mark.parametrize("n,pos,nh,nkv,launches", [(700, 0, 24, 3, 3), (512, 0, 32, 4, 3), (520, 1000, 20, 1, 3), (385, 700, 24, 6, 3), (256, 6000, 16, 2, 4), (520, 4800, 6, 2, 4),
+                                                           (640, 6000, 16, 2, 4)])
+def test_prefill_of_heads_of_128_and_climbing_scores(attn, n, pos, nh, nkv, launches, climb):
+    """The tensor-core kernel at head dim 128, item by item (3 launches: the rows widened, the fast form, the exact form) and in shares (4: their
+    merge), with scores that climb along the prompt by more than the fast form covers: the exact form does those items again."""
+    hd, T = 128, pos + n
+    rows = -(-T // 64) * 64
+    g = gen(n + pos)
+    Q = torch.randn(n, nh, hd, device="cuda", generator=g).to(torch.bfloat16)
+    c = cache_of(1, rows, nkv, hd, 64, "e4m3", seed=n)
+    k, v = rows_of(n, (1, rows, nkv, hd), torch.float32, 0.3), rows_of(n + 1, (1, rows, nkv, hd), torch.float32, 0.3)
+    if climb:
+        k = 0.2 * k + torch.linspace(0, 12, rows, device="cuda")[:, None, None] * torch.sign(Q[n - 1, 0].float())
+    attn.kv8_store(c, k, v, i32([0]))
+    table = torch.tensor(plain.VALUES["e4m3"], device="cuda")
+    k, v = ((table[t.long()] * torch.pow(2.0, s.double() - 127).repeat_interleave(64, 1)[..., None]) for t, s in ((c.k, c.k_scale), (c.v, c.v_scale)))
+    spoil(c, [T])
+    before = attn.ctx.launches
+    got = attn.gqa_prefill_kv8(Q, c, pos)
+    attn.ctx.sync()
+    assert attn.ctx.launches - before == launches
+    limits = pos + 1 + torch.arange(n, device="cuda")
+    want, tol = plain.attend(Q.double(), k[0, :T], v[0, :T], limits, hd ** -0.5, BF16)
+    assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() / tol).max())
+    if climb:       # some row's scores outrun its first tile's by 2^64, which is what flags an item
+        s = (Q[:, 0].double() @ k[0, :T, 0].T).masked_fill(torch.arange(T, device="cuda") >= limits[:, None], -torch.inf) * hd ** -0.5 / np.log(2)
+        assert float((s.amax(1) - s[:, :64].amax(1)).max()) > 100
+
+
+def test_prefill_of_heads_of_128_over_keys_that_leave_l2(attn):
+    """Widened keys and values above 64 MB, items one by one: query tiles of one head after the other."""
+    nh, nkv, hd, n, pos = 148, 4, 128, 128, 40000
+    T = pos + n
+    rows = -(-T // 64) * 64
+    assert 4 * T * nkv * hd > 64 << 20
+    c, k, v = filled(attn, 1, rows, nkv, hd, 64, "int8", seed=2)
+    spoil(c, [T])
+    Q = torch.randn(n, nh, hd, device="cuda", generator=gen(3)).to(torch.bfloat16)
+    before = attn.ctx.launches
+    got = attn.gqa_prefill_kv8(Q, c, pos)
+    attn.ctx.sync()
+    assert attn.ctx.launches - before == 3
+    heads = [0, 36, 37, 74, 147]
+    for h in heads:
+        want, tol = plain.attend(Q[:, h:h + 1].double(), k[0, :T, h // 37:h // 37 + 1], v[0, :T, h // 37:h // 37 + 1],
+                                 pos + 1 + torch.arange(n, device="cuda"), hd ** -0.5, BF16)
+        assert bool(((got[:, h:h + 1].double() - want).abs() <= tol).all()), h
 
 
 def test_a_growing_prompts_workspace_grows_by_doubling(attn):
