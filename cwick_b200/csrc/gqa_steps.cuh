@@ -1,6 +1,6 @@
 // gqa_steps.cuh -- what the streaming GQA decode kernels (gqa_decode.cu: bf16 cache, kv8_decode.cu: 8-bit cache) share: the steps of
-// all sequences dealt out to the blocks in equal contiguous ranges, worked out from the lengths on the device, and the merge of the
-// records that a sequence's blocks leave.
+// all sequences dealt out to the blocks in equal contiguous ranges, worked out from the lengths on the device. (Their records, and the
+// merges of these, are each kernel's own.)
 #pragma once
 #include "cwk_common.cuh"
 
@@ -150,59 +150,6 @@ __device__ __forceinline__ void gqa_advance(const GqaSteps &p, GqaPlace &at) {  
         at.len = length_of(p, at.b);
     } while (at.len <= 0);
     at.steps = steps_of(p, at.b);
-}
-
-// The merge of `cnt` records of one query row, at(i) its i-th {m, l, o[HD]}: (HD / 2) x GROUPS threads, two columns each, the
-// records dealt out to the groups (one sequence has a record from every block: 148 in a row are 20 us of loads for one group of
-// threads). True for the threads of group 0, which get the joined columns x, y (not yet divided) and the sum `den`.
-template <int HD, int GROUPS, class At>
-__device__ __forceinline__ bool gqa_merge_records(int cnt, At at, float &den, float &x, float &y) {
-    constexpr int NT = HD / 2;
-    __shared__ float s_m[GROUPS], s_l[GROUPS];
-    __shared__ float2 s_o[GROUPS][NT];
-    const int g = threadIdx.x / NT, tid = threadIdx.x % NT;
-    float M = -INFINITY;
-    den = x = y = 0.f;
-    for (int i0 = g; i0 < cnt; i0 += 8 * GROUPS) {         // eight records' loads at once; the running maximum as the scores'
-        float m[8], l[8];
-        float2 o[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int i = i0 + j * GROUPS;
-            const float *r = at(min(i, cnt - 1));
-            m[j] = i < cnt ? r[0] : -INFINITY;
-            l[j] = r[1];
-            o[j] = *reinterpret_cast<const float2 *>(r + 2 + 2 * tid);
-        }
-        float mx = M;
-#pragma unroll
-        for (int j = 0; j < 8; j++) mx = fmaxf(mx, m[j]);
-        if (mx == -INFINITY) continue;
-        const float a = exp2f(M - mx);
-        den *= a; x *= a; y *= a;
-        M = mx;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float w = exp2f(m[j] - M);
-            den += w * l[j]; x += w * o[j].x; y += w * o[j].y;
-        }
-    }
-    if (GROUPS > 1) {
-        if (tid == 0) { s_m[g] = M; s_l[g] = den; }
-        s_o[g][tid] = make_float2(x, y);
-        __syncthreads();
-        if (g > 0) return false;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < GROUPS; j++) mx = fmaxf(mx, s_m[j]);
-        den = x = y = 0.f;
-#pragma unroll
-        for (int j = 0; j < GROUPS; j++) {
-            const float w = s_m[j] == -INFINITY ? 0.f : exp2f(s_m[j] - mx);
-            den += w * s_l[j]; x += w * s_o[j][tid].x; y += w * s_o[j][tid].y;
-        }
-    }
-    return true;
 }
 
 }  // namespace

@@ -5,7 +5,7 @@
 // whose scale grows has the codes in front of the new rows rewritten. In front of the quantisation, for cwk_gqa_qk_prep_kv8, keys get
 // their RMS norm and rotation (src/q35_model.c:112-122, :144-153, :459-477), and query heads the same on blocks of their own. Bound: the store by
 // HBM, 16,381 rows of 4 KV heads of 256, bf16 to INT8 (101 MB) 17.8 us = 5.7 TB/s, E4M3 19.0, from f32 28.4 (5.9 TB/s); one row of 64 slots by
-// latency, 2.6 us. The preparation by the instructions of the keys: 7 x 300 rows and 16 query heads (64 MB) 19.6 us, 512 rows 8.2, one
+// latency, 2.6 us. The preparation by the instructions of the keys: 7 x 300 rows and 16 query heads (64 MB) 20.1 us, 512 rows 8.2, one
 // of 64 slots 4.3.
 //
 // Reading is a conversion on the way: the same 16,381 rows to bf16 18.9 us = 5.3 TB/s.
@@ -282,7 +282,7 @@ __device__ __forceinline__ void store_query(uint16_t *dst, const float (&y)[V]) 
 }
 // Those of query heads h0 .. h0 + heads - 1 of a token again, multiplied by a power of two first, and epsilon by its square: large rows (root of the
 // mean 2^49 and up) come below 2^48, small ones are at most 2^44, the least subnormal 2^-49. (Not inlined: to 7 x 300 rows that
-// have no use for it, 19.6 us, it adds 0.9 in line and so 0.5.)
+// have no use for it, 19.6 us, it adds 0.9 in line and so 0.4 to 0.5.)
 template <int V>
 __device__ __noinline__ void query_rows_out_of_range(const Kv8PrepParams &p, int64_t t, int h0, int heads, int lane, const float2 *csf) {
     constexpr int HD = 32 * V;
@@ -612,7 +612,9 @@ int launch_write_rows(cwk_ctx *ctx, PARAMS &p, int type) {
     auto kern = type == CWK_KV8_INT8 ? kv8_write_kernel<V, SRC, true, PARAMS, ROWS> : kv8_write_kernel<V, SRC, false, PARAMS, ROWS>;
     if constexpr (std::is_same<PARAMS, Kv8PrepParams>::value) {
         p.tasks = tasks;
-        p.heads = p.n * (int64_t)p.B * p.nh <= 2048 ? 1 : KQ_HEADS;      // query heads that share a token's angles and are on their way together; few rows: a warp each
+        // Query heads of a token that share its angles and are on their way together; few rows: a warp each. A warp for one / for eight, 16 heads
+        // of 256, replayed: 64 slots 4.4 / 5.0 us, 128 slots 4.6 / 5.3, 256 slots 7.7 / 6.8, 512 tokens of one 11.1 / 9.1.
+        p.heads = p.n * (int64_t)p.B * p.nh <= 2048 ? 1 : KQ_HEADS;
         blocks += ((int64_t)p.B * p.n * ((p.nh + p.heads - 1) / p.heads) + warps - 1) / warps;
         smem = (size_t)(p.rot / 2) * warps * ROWS * sizeof(float2);      // 128 KB at most (32 KB for 64 values in blocks of 128 rows)
         static bool attr_set[2][16] = {};

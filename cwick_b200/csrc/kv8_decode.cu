@@ -10,9 +10,11 @@
 //   values   ldmatrix.trans on pairs of bytes gives a lane two keys of two neighbouring columns; one byte permutation pairs the keys, and
 //            the even column goes to row g of the MMA, the odd one to row g + 8.
 // The queries go to f16 too: each row divided by a power of two that brings its largest value into [1, 2), so what is lost is below
-// 2^-25 of that value, 2^-16 of a bf16 step. Probabilities are f16 in [0, 2^8], three bits finer than bf16's; their sums are f32. The
-// scales are powers of two: a step's 32 keys are in one block, the key scale multiplies its scores and the value scale its product
-// on the way into the f32 accumulators, so no code's value is ever rounded or out of f16's range.
+// 2^-25 of that value, 2^-16 of a bf16 step. Probabilities are f16 in [0, 2^8], three bits finer than bf16's from 2^-14 up; below, the
+// step stays 2^-24, and one under 2^-25 is zero in the product while the f32 sum counts it: 10,000 such keys of a warp are 3e-4 of its
+// largest, a thirteenth of the result's own rounding. The sums are f32. The scales are powers of two: a step's 32 keys are in one
+// block, the key scale multiplies its scores and the value scale its product on the way into the f32 accumulators, so no code's value
+// is ever rounded or out of f16's range.
 //
 // What bounds it: a batch by HBM, 64 sequences of 4096 rows (16 heads, 4 KV heads of 256, 537 MB) 91 us = 5.9 TB/s, INT8 the same, four tokens each 110;
 // less by the start and the end of the streams, 16 sequences 32 us, one 8.4, of 32768 rows 21 (replayed); short caches by a warp's chain of steps,

@@ -1474,9 +1474,10 @@ int cwk_mla_prefill_attn_tc(cwk_ctx *ctx, const void *Q, const float *rot, const
 }
 
 // Causal GQA prefill on the same kernel (Qwen3.5 full-attention layers, src/q35_model.c:1713-1746): per query head,
-// 128 consecutive queries are the MMA's rows; keys and values are the 256-wide rows of the head's KV head, streamed in
-// 64-key tiles by TMA straight from the caches. Q bf16 [n][nh][256]; K, V bf16 [pos + n][nkv][256]; out bf16
-// [n][nh][256]; flags = workspace int32 [ceil(n / 128) * nh + number of SMs + 3]. Returns CWK_ERR_UNSUPPORTED (no error text) when the
+// 128 consecutive queries are the MMA's rows; keys and values are the rows of the head's KV head, 256 or 128 wide, streamed in
+// 64-key tiles by TMA straight from the caches. Q bf16 [n][nh][hd]; K, V bf16 [pos + n][nkv][hd]; out bf16
+// [n][nh][hd]; flags = workspace int32 [ceil(n / 128) * nh + number of SMs + 3]; spread: items go out from the longest of all heads to the
+// shortest, for K and V that stay in L2 (where items are shared it changes nothing). Returns CWK_ERR_UNSUPPORTED (no error text) when the
 // tensor path cannot take the operands.
 int cwk_gqa_prefill_tc(cwk_ctx *ctx, const void *Q, const void *K, const void *V, int64_t pos, int n, int nh, int nkv, int hd,
                        float scale, void *out, int *flags, int spread) {

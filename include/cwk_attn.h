@@ -306,13 +306,14 @@ CWK_API int cwk_kv8_load(cwk_ctx *ctx, const cwk_kv8 *cache, const int32_t *pos,
 /* cwk_gqa_qk_prep for B slots at positions of their own and this cache: RMS norm with (1 + w) weights of query and key heads, rotate-half
  * RoPE on the first `rot` values (a multiple of 16), queries to bf16, keys and values into the cache as cwk_kv8_store does. qg f32
  * [B][n][nh][2*hd] (q | gate per head), k, v f32 [B][n][nkv][hd], q_norm, k_norm f32 [hd], q_out bf16 [B][n][nh][hd]. pos, count as above;
- * the query rows of tokens from count[b] on are left as they were. Angles, and keys up to their code, are formed in double. */
+ * the query rows of tokens from count[b] on, and of tokens that have no row in the slot, are left as they were. Angles, and keys up to their code, are
+ * formed in double, queries in float. */
 CWK_API int cwk_gqa_qk_prep_kv8(cwk_ctx *ctx, const float *qg, const float *k, const float *v, const float *q_norm, const float *k_norm, float eps,
                                 int rot, double theta, const int32_t *pos, const int32_t *count, int B, int n, int nh, void *q_out,
                                 const cwk_kv8 *cache);
 /* cwk_gqa_decode over this cache, for n >= 1 query tokens per sequence: the last n of the kv_len[b] rows are those of the query tokens, token
- * i sees rows 0 .. kv_len[b] - n + i (none: zeros). q, out bf16 [B][n][nh][hd], sequence b in slot b, kv_len int32 [B] device, at most max_kv_len
- * (a larger one counts as the slot's rows), nh / nkv at most 16. Up to 16 / (nh / nkv) tokens share a pass over the cache. */
+ * i sees rows 0 .. kv_len[b] - n + i (none: zeros). q, out bf16 [B][n][nh][hd], sequence b in slot b, kv_len int32 [B] device (beyond the slot's
+ * rows: as those); max_kv_len, at most the slot's rows, is the longest that is expected, by which the launch is shaped; nh / nkv at most 16. Up to 16 / (nh / nkv) tokens share a pass over the cache. */
 CWK_API int cwk_gqa_decode_kv8(cwk_ctx *ctx, const void *q, const cwk_kv8 *cache, const int32_t *kv_len, int max_kv_len, int B, int n, int nh,
                                float scale, void *out, int n_splits);
 /* cwk_gqa_prefill over this cache: queries at positions pos .. pos + n - 1 of one slot against its first pos + n rows.

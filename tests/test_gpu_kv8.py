@@ -410,6 +410,23 @@ def test_decode_of_sequences_of_nan_rows(attn, n, lens, n_splits):
         assert bool(got[1:].isfinite().all())
 
 
+
+@pytest.mark.parametrize("expected", [0, 32, 1024])
+@pytest.mark.parametrize("B,n,n_splits", [(3, 1, 0), (3, 5, 0), (3, 1, 2), (70, 1, 0)])
+def test_decode_of_lengths_beyond_what_was_expected(attn, B, n, n_splits, expected):
+    """max_kv_len shapes the launch only: longer sequences are read to their end, and a length beyond the slot's rows is the slot's."""
+    nh, nkv, hd, rows = 16, 4, 256, 1024
+    c, k, v = filled(attn, B, rows, nkv, hd, 64, "int8", seed=6)
+    q = torch.randn(B, n, nh, hd, device="cuda", generator=gen(6)).to(torch.bfloat16)
+    lens = [1000, 2 ** 31 - 1, 7, 1025, -3] * 14
+    got = attn.gqa_decode_kv8(q, c, i32(lens[:B]), max_kv_len=expected, n_splits=n_splits)
+    attn.ctx.sync()
+    for b in range(B):
+        m = min(max(lens[b], 0), rows)
+        want, tol = plain.attend(q[b].double(), k[b, :m], v[b, :m], (m - n + 1 + torch.arange(n, device="cuda")).clamp(min=0), hd ** -0.5, F16)
+        assert bool(((got[b].double() - want).abs() <= tol).all()), b
+
+
 def test_decode_gives_the_same_bits_again(attn):
     c, k, v = filled(attn, 3, 1024, 4, 256, 64, "e4m3", seed=8)
     q = torch.randn(3, 16, 256, device="cuda", generator=gen(2)).to(torch.bfloat16)
