@@ -526,6 +526,7 @@ namespace {
 struct Kv8Shape {
     int hb, per, parts, keys, cols, blocks;
     int64_t groups;
+    int64_t places;       // for records, a block's warps each, if the steps go out in shares
     bool whole;
     double us;
     Kv8Shape(int sm_count, int B, int64_t len, int n, int nh, int nkv, int hd, int max_blocks) {
@@ -556,6 +557,7 @@ struct Kv8Shape {
             if (x < one) { one = x; alone = each * step(1) + ends; best = h; }
         }
         const int64_t each = deal(nkv % 4 == 0 ? 4 : nkv % 2 == 0 ? 2 : 1), steps = B * groups * each;
+        places = B * groups + slots;
         // as many blocks as there can be steps, at most two per SM
         blocks = (int)std::min<int64_t>(std::max<int64_t>(1, steps), max_blocks > 0 ? std::min<int64_t>(max_blocks, slots) : slots);
         const double turns = (double)((steps + blocks - 1) / blocks), records = (double)blocks * GW * cols * hd * 4e-6;
@@ -606,13 +608,15 @@ int cwk_kv8_streams(cwk_ctx *ctx, const void *q, const cwk_kv8 &c, const int32_t
     p.out = (uint16_t *)out;
     p.steps = GqaSteps{kv_len, B, (int)shape.groups, shape.keys, kv_len ? (int)c.rows : max_kv_len, nullptr};
     const bool two = shape.cols > 8;
+    // Whole blocks have no records. Their room is there all the same, so that it grows with the sequences and the tokens alone: a context that
+    // has done the largest of its steps has it for every smaller one, captured or not.
+    const size_t rec_bytes = (size_t)shape.places * GW * kv8_record(shape.cols, c.hd) * sizeof(float);
+    const int s = cwk_reserve_scratch(ctx, rec_bytes + (size_t)shape.places * sizeof(int2));
+    if (s != CWK_OK) return s;
     if (shape.whole) {
         if (c.hd == 256) return two ? launch<256, 2, true>(ctx, p, c.type, blocks) : launch<256, 1, true>(ctx, p, c.type, blocks);
         return two ? launch<128, 2, true>(ctx, p, c.type, blocks) : launch<128, 1, true>(ctx, p, c.type, blocks);
     }
-    const size_t rec_bytes = (size_t)(B * shape.groups + blocks) * GW * kv8_record(shape.cols, c.hd) * sizeof(float);
-    const int s = cwk_reserve_scratch(ctx, rec_bytes + (size_t)B * shape.groups * sizeof(int2));
-    if (s != CWK_OK) return s;
     p.rec = ctx->scratch;
     p.steps.meta = (int2 *)((uint8_t *)ctx->scratch + rec_bytes);
     if (c.hd == 256) return two ? launch<256, 2, false>(ctx, p, c.type, blocks) : launch<256, 1, false>(ctx, p, c.type, blocks);

@@ -59,7 +59,9 @@ typedef struct cwk_ctx cwk_ctx;
  * therefore only valid until a LARGER call runs on the same context: warm the
  * context up with the largest shape before capturing, and do not grow it while
  * a captured graph is still being replayed (nor during capture, which an
- * allocation would break). */
+ * allocation would break). Where a call's form depends on its sizes (prompt
+ * chunks, bf16 GQA decode), a smaller call may need a buffer that the largest
+ * does not: there, warm up with every shape that is captured. */
 CWK_API int cwk_ctx_create(int device, cwk_ctx **out);
 CWK_API void cwk_ctx_destroy(cwk_ctx *ctx);
 /* Run on a caller-owned cudaStream_t instead of the context's own. */

@@ -427,6 +427,44 @@ def test_decode_of_lengths_beyond_what_was_expected(attn, B, n, n_splits, expect
         assert bool(((got[b].double() - want).abs() <= tol).all()), b
 
 
+
+@pytest.mark.parametrize("largest,smaller", [((64, 1200, 1), [(16, 1200, 1), (16, 2000, 1)]), ((16, 500, 4), [(1, 4000, 4), (12, 900, 3), (2, 3000, 1)])])
+def test_decode_captured_after_the_largest_step(attn, largest, smaller):
+    """A context that has done the largest step has room for smaller ones, although the largest takes a form without records: their capture
+    takes no memory, and one's replay holds after the others."""
+    from cwick_b200.ops import Attn
+    nh, nkv, hd = 16, 4, 256
+    rows = max(x[1] for x in [largest] + smaller)
+    rows = -(-rows // 64) * 64
+    c, _, _ = filled(attn, largest[0], rows, nkv, hd, 64, "e4m3", seed=9)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def query(B, n):
+        return torch.randn(B, n, nh, hd, device="cuda", generator=gen(B)).to(torch.bfloat16)
+    with torch.cuda.stream(side):
+        a = Attn(0)
+        before = a.ctx.launches
+        a.gqa_decode_kv8(query(largest[0], largest[2]), c, i32([largest[1]] * largest[0]), max_kv_len=largest[1])
+        assert a.ctx.launches - before == 1               # whole blocks
+        graphs = []
+        for B, length, n in smaller:
+            q, lens = query(B, n), i32([length] * B)
+            torch.cuda.synchronize()                      # (the other context is on another stream)
+            out, want = torch.empty_like(q), attn.gqa_decode_kv8(q, c, lens, max_kv_len=length)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                a.gqa_decode_kv8(q, c, lens, max_kv_len=length, out=out)
+            graphs.append((graph, out, want, q, lens))    # (the graph reads these two)
+        for graph, out, want, *_ in graphs + graphs[::-1]:
+            out.zero_()
+            graph.replay()
+            side.synchronize()
+            assert torch.equal(out, want)
+    del graphs, graph
+
+
 def test_decode_gives_the_same_bits_again(attn):
     c, k, v = filled(attn, 3, 1024, 4, 256, 64, "e4m3", seed=8)
     q = torch.randn(3, 16, 256, device="cuda", generator=gen(2)).to(torch.bfloat16)
